@@ -13,7 +13,7 @@ in the step; ``context``: tokens of a request behind the step (the mean; ``ragge
 A cached row of ``dh`` numbers is held as e4m3 numbers times a power of two of its own, the smallest with which the row's
 largest magnitude stays within 448 (a byte: the exponent plus 127, from 1 on).  A page is ``[hk, 2, page, dh]`` codes and
 ``[hk, 2, page]`` scale bytes; the codes of sixteen keys lie together in pieces of 64 elements (a last piece of 32 where 64
-does not divide the head), keys key by key, values with four keys of an element side by side (:func:`places`).
+does not divide the head), in the order in which a matrix instruction's lanes take them (:func:`places`).
 """
 import math
 
@@ -223,9 +223,10 @@ def places(dh, device):
     """Where element ``d`` of key ``j`` of sixteen lies among their ``16 * dh`` codes, ``[16, dh]``: keys, values."""
     j = torch.arange(16, device=device)[:, None]
     d = torch.arange(dh, device=device)[None, :]
-    piece = (dh - d // 64 * 64).clamp(max=64)
+    u = (dh - d // 64 * 64).clamp(max=64) // 4  # codes that a lane takes
     start = d // 64 * 1024
-    return start + j * piece + d % 64, start + d % 16 * piece + j // 4 * (piece // 4) + d % 64 // 16 * 4 + j % 4
+    return (start + d % 64 // u * 16 * u + j * u + d % u,
+            start + j // 4 * 16 * u + d % 16 * u + d % 64 // 16 * 4 + j % 4)
 
 
 def plain_rows(codes, scales):
@@ -395,8 +396,8 @@ def exact_rows(s, ids, h, which):
     for d0 in range(0, dh, 64):
         w = min(64, dh - d0)
         piece = x[:, 16 * d0: 16 * (d0 + w)]
-        if which == 0:
-            out[:, :, d0: d0 + w] = piece.view(-1, 16, w)
-        else:  # [element % 16, key / 4, element / 16, key % 4]
-            out[:, :, d0: d0 + w] = piece.view(-1, 16, 4, w // 16, 4).permute(0, 2, 4, 3, 1).reshape(-1, 16, w)
+        if which == 0:  # [a quarter of the elements, key, element]
+            out[:, :, d0: d0 + w] = piece.view(-1, 4, 16, w // 4).transpose(1, 2).reshape(-1, 16, w)
+        else:  # [key / 4, element % 16, element / 16, key % 4]
+            out[:, :, d0: d0 + w] = piece.view(-1, 4, 16, w // 16, 4).permute(0, 1, 4, 3, 2).reshape(-1, 16, w)
     return out.view(-1, dh) * torch.exp2(s.scales[ids, h, which].double() - 127.0).reshape(-1, 1)
