@@ -17,6 +17,8 @@ from torch.autograd import forward_ad
 from torch.utils._device import DeviceContext
 
 from . import build as _build
+from . import quantized as _quantized
+from .quantized import QuantizedPages
 from .transfer import to_device
 
 # the rules under which the attention kernels here read keys ("window_keep": the general kernel alone)
@@ -130,6 +132,10 @@ _SIGNATURES = {
     "jle_attention_prefill_kept": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _vp, _i, _i, _i, _f, _i, _i, _i, _i, _vp],
     "jle_paged_attention_kept": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _f, _i, _i, _i, _i, _i, _i, _i, _i, _vp,
                                  _vp, _vp],
+    "jle_quantized_prepare": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _vp, _vp, _i, _i, _f, _f, _i, _i, _i, _i, _i, _i, _vp],
+    "jle_quantized_read": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
+    "jle_attention_quantized": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i,
+                                _i, _vp],
     "jle_paged_attention_biased": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _i, _i, _i, _i, _i, _i, _i, _i, _vp,
                                    _vp, _vp, _i, _vp, _f, _vp],
 }
@@ -2111,7 +2117,10 @@ class HipOps:
 
     # ------------------------------------------------------------------ attention
     def qk_prepare_kv_write(self, qkv, num_heads, num_kv_heads, head_dim, positions, prep, kv_cache, slot_mapping):
-        """``prep``: a :class:`~..parts.base.QKPreparation`."""
+        """``prep``: a :class:`~..parts.base.QKPreparation`.  ``kv_cache``: pages in the run dtype, or
+        :class:`~.quantized.QuantizedPages` (bfloat16 rows; keys and values are then rounded once, to 8 bits)."""
+        if isinstance(kv_cache, QuantizedPages):
+            return self._qk_prepare_quantized(qkv, num_heads, num_kv_heads, head_dim, positions, prep, kv_cache, slot_mapping)
         n = qkv.shape[0]
         hq, hk, dh = num_heads, num_kv_heads, head_dim
         self._chk(qkv, None, (n, (hq + 2 * hk) * dh), "q|k|v")
@@ -2192,6 +2201,10 @@ class HipOps:
         """From the fused q|k|v rows to the attention output ``[N, num_heads * head_dim]``: q and k prepared as
         ``prep`` says, k and v written into their pages (if this run ``writes`` its cache), attention over the
         pages.  A step of single tokens in bfloat16 is one launch (``attention_decode_fused_kernel``)."""
+        if isinstance(kv_cache, QuantizedPages):
+            q = self._qk_prepare_quantized(qkv, num_heads, num_kv_heads, head_dim, positions, prep, kv_cache, slot_mapping,
+                                           writes)
+            return self.paged_attention(q, kv_cache, block_table, positions, token_segment, retention, scale, meta)
         n = qkv.shape[0]
         hq, hk, dh = num_heads, num_kv_heads, head_dim
         ps = kv_cache.shape[3]
@@ -2261,14 +2274,14 @@ class HipOps:
         return whole
 
     def attention_plan(self, seg_lens, seg_starts, retention, device, num_kv_heads=1, group_size=1, decode_bucket=None,
-                       tile=None, single_tiles=False):
+                       tile=None, single_tiles=False, at_least=1):
         """Work lists of the MFMA attention kernels for one step and one retention rule: the rows that are
         single decode tokens (and into how many keys their work is split; ``single_tiles``: these are tiles too), tiles of up
         to 32 consecutive tokens of longer segments and, with ``group_size`` > 1 query heads per kv head, the packing of the
         (tile, head) items of a kv head into blocks of wavefronts that share keys.  ``decode_bucket``: the step
         holds single tokens only, none beyond this context length: the split is then chosen from the number of
         tokens and this bound alone (not from where each request stands), so the same launch fits every such
-        step."""
+        step.  ``at_least``: segments of fewer tokens are left to another kernel."""
         from ..parts.base import first_needed_position
 
         # (plain lists: of up to tens of segments they are laid out in half the time of arrays, 12 us a portion of 77 tokens)
@@ -2276,7 +2289,9 @@ class HipOps:
         tile = tile or self.PREFILL_TILE
         o = 0
         for i, n in enumerate(seg_lens):
-            if n == 1 and not single_tiles:
+            if n < at_least:
+                pass
+            elif n == 1 and not single_tiles:
                 dec.append(o)
                 if decode_bucket is None:
                     spans.append((first_needed_position(retention, seg_starts[i]), seg_starts[i]))
@@ -2353,7 +2368,11 @@ class HipOps:
         """``bias``: float32 ``[Hq, L]``: a key ``n`` places back adds ``bias[h, min(n, L - 1)]`` to head ``h``'s scaled
         score; ``sink``: float32 ``[Hq]``: ``exp(sink[h])`` is one more term of head ``h``'s denominator; ``penalty``:
         float32 ``[Hq, 2]``: ``penalty[h, 0] * ln(1 + penalty[h, 1] * n)`` is taken off (without a ``bias``); ``cap``: a scaled
-        score ``s`` becomes ``cap tanh(s / cap)`` (without either)."""
+        score ``s`` becomes ``cap tanh(s / cap)`` (without either).  Over pages in 8 bits: none of these."""
+        if isinstance(kv_cache, QuantizedPages):
+            if bias is not None or sink is not None or penalty is not None or cap is not None:
+                raise KernelError("attention over a cache in 8 bits takes no distance table, sinks, penalty or score cap")
+            return self._attention_quantized(q, kv_cache, block_table, positions, token_segment, retention, scale, meta)
         n, hq, dh = q.shape
         hk, ps = kv_cache.shape[2], kv_cache.shape[3]
         self._chk(q, kv_cache.dtype, None, "q")
@@ -2532,6 +2551,184 @@ class HipOps:
         self._call("jle_paged_attention_kept", _p(q), _p(kv_cache), _p(out), _p(positions), _p(token_segment),
                    _p(block_table), block_table.shape[1], mode, param, keep, float(scale), self._is_bf16(q), n, hq, hk,
                    dh, ps, splits, tiles_per_split, _p(ws_ml), _p(ws_o))
+        return out
+
+    # ------------------------------------------------------------------ keys and values in 8 bits
+    def _chk_quantized(self, kv, num_heads: int, num_kv_heads: int, head_dim: int) -> None:
+        self._chk(kv.codes, torch.uint8, None, "codes")
+        if kv.device != self._tickets.device:
+            raise KernelError(f"pages on {kv.device}, the kernels run on {self._tickets.device}")
+        if kv.shape[2] != num_kv_heads or kv.shape[4] != head_dim:
+            raise KernelError(f"pages of {kv.shape[2]} kv heads of {kv.shape[4]}, asked for {num_kv_heads} of {head_dim}")
+        try:
+            _quantized.check_sizes(num_heads, num_kv_heads, head_dim, kv.shape[3])
+        except ValueError as e:
+            raise KernelError(str(e)) from None
+
+    def _chk16(self, t, dtype, shape, what: str):
+        self._chk(t, dtype, shape, what)
+        if t.device != self._tickets.device:
+            raise KernelError(f"{what} on {t.device}, the kernels run on {self._tickets.device}")
+        if t.data_ptr() % 16:
+            raise KernelError(f"{what} must be aligned to 16 bytes")
+        return t
+
+    def _qk_prepare_quantized(self, qkv, num_heads, num_kv_heads, head_dim, positions, prep, kv, slot_mapping,
+                              writes: bool = True):
+        n = qkv.shape[0]
+        hq, hk, dh = num_heads, num_kv_heads, head_dim
+        self._chk_quantized(kv, hq, hk, dh)
+        self._chk16(qkv, torch.bfloat16, (n, (hq + 2 * hk) * dh), "q|k|v (for a cache in 8 bits)")
+        self._chk(positions, torch.int32, (n,), "positions")
+        if writes:
+            self._chk(slot_mapping, torch.int32, (n,), "slot mapping")
+        if prep.norm_span != "head":
+            raise KernelError("queries and keys for a cache in 8 bits are normed head by head")
+        rot, inv_freq, pairing, rd = prep.rotation, None, 0, 0
+        if rot is not None:
+            inv_freq, rd = rot.inv_freq, int(rot.rotary_dim) or dh
+            if rot.pairing not in ("adjacent", "half") or float(rot.magnitude) != 1.0:
+                raise KernelError("a cache in 8 bits takes adjacent or half-split pairs, sines and cosines as they are")
+            pairing = 0 if rot.pairing == "adjacent" else 1
+            if not 0 < rd <= dh or rd % (16 if pairing else 2):
+                raise KernelError(f"rotary/norm kernel: {rd} rotated elements of a head of {dh} (half-split pairs: a multiple "
+                                  "of 16)")
+            self._chk(inv_freq, torch.float32, (rd // 2,), "inv_freq")
+        for w, what in ((prep.norm_weight_q, "q norm weight"), (prep.norm_weight_k, "k norm weight")):
+            if w is not None:
+                if prep.norm_eps is None:
+                    raise KernelError("rotary/norm kernel: norm weights without a norm")
+                self._chk(w, torch.float32, (dh,), what)
+        q = torch.empty(n, hq, dh, dtype=qkv.dtype, device=qkv.device)
+        fs, sc = (prep.query_scale if prep.query_scale is not None else (0.0, 0.0))
+        self._call("jle_quantized_prepare", _p(qkv), _p(q), _p(kv.codes) if writes else None,
+                   _p(kv.scales) if writes else None, _p(positions), _p(slot_mapping) if writes else None, _p(inv_freq),
+                   -1.0 if prep.norm_eps is None else float(prep.norm_eps), int(bool(prep.norm_first)),
+                   _p(prep.norm_weight_q), _p(prep.norm_weight_k), pairing, rd, float(fs), float(sc), n, hq, hk, dh,
+                   kv.shape[3], kv.shape[0])
+        return q
+
+    def read_pages(self, kv: QuantizedPages, page_ids):
+        """The given pages (int32, on the device) of a cache in 8 bits, in bfloat16 and in the layout in which the attention
+        kernels read pages, ``[n, 2, kv_heads, page_size, head_dim]``; every number is exact.  An id that is no page's gives
+        NaN."""
+        self._chk(page_ids, torch.int32, (page_ids.numel(),), "page ids")
+        return self._read_pages(kv, page_ids, None)
+
+    def _read_pages(self, kv, page_ids, where):
+        """``where``: the places of ``page_ids`` that are meant (all, one after the other)."""
+        p, _, hk, ps, dh = kv.shape
+        self._chk_quantized(kv, hk, hk, dh)
+        if p == 0:
+            raise KernelError("no pages to read")
+        n = page_ids.numel() if where is None else where.numel()
+        out = torch.empty(n, 2, hk, ps, dh, dtype=torch.bfloat16, device=kv.device)
+        self._call("jle_quantized_read", _p(kv.codes), _p(kv.scales), _p(page_ids), _p(where), _p(out), n, p, hk, dh, ps)
+        return out
+
+    QUANTIZED_COLUMNS = 64  # a segment whose tokens times query heads a kv head are no more takes the kernel over codes
+    QUANTIZED_STEPS = (256, 4096)  # keys of a block's range: at least, at most
+    QUANTIZED_KEY_US, QUANTIZED_MERGE_US, QUANTIZED_RESULT_US = 0.02, 4.0, 0.05
+
+    def _quantized_plan(self, seg_lens, seg_starts, retention, num_kv_heads: int, group: int, head_dim: int, page_size: int,
+                        decode_bucket, block_table):
+        """What a step's attention over pages in 8 bits is made of.  ``few``: for segments of few tokens, by the columns that
+        a wavefront takes (16, 32, 64), ``(tiles, number, columns, ranges, keys a range)``; ``long``: for the others, the
+        tiles of the attention kernel over pages in bfloat16, the pages it needs read back and the block table over those."""
+        from ..parts.base import first_needed_position
+
+        device = block_table.device
+        if block_table.numel() >= 1 << 31:
+            raise KernelError("a block table of 2^31 places and more")
+        most = min(self.QUANTIZED_COLUMNS, 32 if head_dim == 256 else 64)
+        tokens = max(1, most // group)
+        few = {}
+        o = 0
+        for i, n in enumerate(seg_lens):
+            if n <= tokens:
+                cols = 16 if n * group <= 16 else 32 if n * group <= 32 else 64
+                start = None if seg_starts is None else seg_starts[i]
+                few.setdefault(cols, []).append((o, n, start))
+            o += n
+        plan = {"few": [], "long": None}
+        for cols, items in sorted(few.items()):
+            if decode_bucket is not None:
+                of = lambda cand: [self._most_ranges(retention, decode_bucket, cand)] * len(items)
+            else:
+                spans = [(first_needed_position(retention, s), s + n - 1) for _, n, s in items]
+                of = lambda cand: [last // cand - first // cand + 1 for first, last in spans]
+            best = None
+            low, high = self.QUANTIZED_STEPS
+            cand = low
+            while cand <= high:
+                r = of(cand)
+                blocks = num_kv_heads * sum(r)
+                cost = (-(-blocks // self._compute_units) * cand * self.QUANTIZED_KEY_US
+                        + (self.QUANTIZED_MERGE_US + self.QUANTIZED_RESULT_US * max(r) if max(r) > 1 else 0.0))
+                if best is None or cost <= best[0]:
+                    best = (cost, cand, max(r))
+                cand += low
+            flat = [x for at, n, _ in items for x in (at, n)]
+            plan["few"].append((to_device(torch.from_numpy(np.array(flat, np.int32)), device), len(items),
+                                max(n for _, n, _ in items) * group, best[2], best[1]))
+        if any(n > tokens for n in seg_lens):
+            ps, width = page_size, block_table.shape[1]
+            where = []
+            for i, n in enumerate(seg_lens):
+                if n > tokens:
+                    first = first_needed_position(retention, seg_starts[i]) // ps
+                    last = min((seg_starts[i] + n - 1) // ps, width - 1)
+                    where.append(np.arange(i * width + first, i * width + last + 1, dtype=np.int32))
+            where = np.concatenate(where)
+            table = np.full(block_table.numel(), -1, np.int32)
+            table[where] = np.arange(where.size, dtype=np.int32)
+            sent = to_device(torch.from_numpy(np.concatenate([where, table])), device)
+            where, table = sent[: where.size], sent[where.size:].view(block_table.shape)
+            tiles = self.attention_plan(seg_lens, seg_starts, retention, device, num_kv_heads, group, single_tiles=True,
+                                        at_least=tokens + 1)
+            plan["long"] = (tiles, where, table)
+        return plan
+
+    def _attention_quantized(self, q, kv, block_table, positions, token_segment, retention, scale: float, meta):
+        n, hq, dh = q.shape
+        p, _, hk, ps, _ = kv.shape
+        self._chk_quantized(kv, hq, hk, dh)
+        self._chk16(q, torch.bfloat16, (n, hq, dh), "q (over a cache in 8 bits)")
+        self._chk(block_table, torch.int32, None, "block table")
+        self._chk(positions, torch.int32, (n,), "positions")
+        self._chk(token_segment, torch.int32, (n,), "token segments")
+        if retention[0] == "window_keep":
+            raise KernelError("attention over a cache in 8 bits reads keys under the rules all, chunk and window")
+        if not scale > 0:
+            raise KernelError("attention over a cache in 8 bits takes a positive softmax scale")
+        mode = _ret_mode(retention)
+        param = int(retention[1]) if len(retention) > 1 else 0
+        out = torch.empty(n, hq * dh, dtype=q.dtype, device=q.device)
+        if n == 0:
+            return out
+        key = ("quantized_plan", tuple(retention), hk, hq // hk, dh, ps)
+        plan = meta.meta.get(key) if meta is not None else None
+        if plan is None:
+            bucket = meta.decode_bucket if meta is not None else None
+            seg_lens, seg_starts = (meta.seg_lens, None) if bucket is not None else self._segments(meta, token_segment, positions)
+            plan = self._quantized_plan(seg_lens, seg_starts, retention, hk, hq // hk, dh, ps, bucket, block_table)
+            if meta is not None:
+                meta.meta[key] = plan
+        for tiles, num, cols, ranges, span in plan["few"]:
+            ws_ml = ws_o = None
+            if ranges > 1:
+                slots = num * hk * ranges * cols
+                ws_ml = torch.empty(slots * 2, dtype=torch.float32, device=q.device)
+                ws_o = torch.empty(slots * dh, dtype=torch.float32, device=q.device)
+            self._call("jle_attention_quantized", _p(q), _p(kv.codes), _p(kv.scales), _p(out), _p(ws_ml), _p(ws_o),
+                       _p(positions), _p(token_segment), _p(block_table), block_table.shape[1], p, _p(tiles), num, cols,
+                       ranges, span, mode, param, float(scale), hq, hk, dh, ps)
+        if plan["long"] is not None:
+            tiles, where, table = plan["long"]
+            pages = self._read_pages(kv, block_table, where)
+            self._call("jle_attention_prefill", _p(q), _p(pages), _p(out), _p(positions), _p(token_segment), _p(table),
+                       table.shape[1], _p(tiles["tiles"]), tiles["num_tiles"], self.PREFILL_TILE, _p(tiles["groups"]),
+                       tiles["num_groups"], mode, param, float(scale), hq, hk, dh, ps, None, 0, None, 0.0)
         return out
 
     # ------------------------------------------------------------------ routed experts

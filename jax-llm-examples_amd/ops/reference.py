@@ -15,6 +15,7 @@ from typing import Optional
 
 import torch
 
+from .quantized import QuantizedPages, read_pages, read_rows, store_rows
 
 def retention_start(retention: tuple, pos: torch.Tensor) -> torch.Tensor:
     """First key position a query at ``pos`` may read (vectorised)."""
@@ -650,7 +651,8 @@ class ReferenceOps:
         ``1 + attn_scale * ln(1 + floor((pos + 1) / floor_scale))``.  Then k and v are written into
         their page at ``slot = page * page_size + offset``.  ``kv_cache`` is ``[pages, 2, kv_heads,
         page_size * head_dim]`` in memory: plane 0 holds keys as ``[page_size, head_dim]``, plane 1
-        holds values transposed, ``[head_dim, page_size]``.  Returns q ``[N, num_heads, head_dim]``."""
+        holds values transposed, ``[head_dim, page_size]``; or it is
+        :class:`~.quantized.QuantizedPages`.  Returns q ``[N, num_heads, head_dim]``."""
         n = qkv.shape[0]
         dt = qkv.dtype
         hq, hk, dh = num_heads, num_kv_heads, head_dim
@@ -689,7 +691,9 @@ class ReferenceOps:
             floor_scale, attn_scale = prep.query_scale
             s = 1.0 + attn_scale * torch.log1p(torch.floor((positions.float() + 1.0) / floor_scale))
             q = q * s[:, None, None]
-        if kv_cache is not None:
+        if isinstance(kv_cache, QuantizedPages):
+            store_rows(kv_cache, k, v, slot_mapping)
+        elif kv_cache is not None:
             ps = kv_cache.shape[3]
             page = (slot_mapping // ps).long()
             off = (slot_mapping % ps).long()
@@ -727,6 +731,10 @@ class ReferenceOps:
             values_t(kv_cache)[page, :, :, off] = pad(v).to(kv_cache.dtype)
         return pad(q.reshape(n, hq, dk)).to(dt).contiguous()
 
+    def read_pages(self, kv, page_ids, dtype=torch.bfloat16):
+        """The given pages of a cache in 8 bits in the run dtype's layout (see :func:`~.quantized.read_pages`)."""
+        return read_pages(kv, page_ids, dtype)
+
     def attention_from_qkv(self, qkv, num_heads, num_kv_heads, head_dim, positions, token_segment, prep, kv_cache,
                            writes: bool, slot_mapping, block_table, retention, scale: float, meta=None):
         """q and k prepared, k and v written (if this run writes its cache), attention over the pages."""
@@ -746,6 +754,7 @@ class ReferenceOps:
         n, hq, dh = q.shape
         hk, ps = kv_cache.shape[2], kv_cache.shape[3]
         g = hq // hk
+        held = isinstance(kv_cache, QuantizedPages)
         out = torch.empty(n, hq * dh, dtype=q.dtype, device=q.device)
         keep = 0
         if retention[0] == "window_keep":  # the window's keys and the sequence's first `keep` tokens
@@ -761,8 +770,12 @@ class ReferenceOps:
             if bool((pages < 0).any()):
                 raise RuntimeError(f"token {i} at position {p} reads a page that was given back")
             off = (kpos % ps).long()
-            k = kv_cache[pages, 0, :, off].float()  # [T, hk, dh]
-            v = values_t(kv_cache)[pages, :, :, off].float()
+            if held:
+                which, place = torch.unique(pages, return_inverse=True)
+                k, v = (x.transpose(1, 2)[place, off] for x in read_rows(kv_cache, which))
+            else:
+                k = kv_cache[pages, 0, :, off].float()  # [T, hk, dh]
+                v = values_t(kv_cache)[pages, :, :, off].float()
             qi = q[i].float().reshape(hk, g, dh)
             sc = torch.einsum("hgd,thd->hgt", qi, k) * scale
             if cap is not None:

@@ -1,0 +1,381 @@
+"""A cache of keys and values in 8 bits: the format, writing, reading back, attention over it, and an engine that keeps its
+cache so.  The oracles are plain 64-bit statements."""
+import math
+
+import pytest
+import torch
+
+from jax_llm_examples_amd.engine.batch import GroupContext, decode_bucket
+from jax_llm_examples_amd.ops import quantized as Q
+from jax_llm_examples_amd.ops.quantized import QuantizedPages
+from jax_llm_examples_amd.ops.reference import ReferenceOps
+from jax_llm_examples_amd.parts.base import QKPreparation, Rotation
+
+gpu = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from jax_llm_examples_amd.engine import get_ops
+    return get_ops(DEV)
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ------------------------------------------------------------------------------------------------ the format
+def held(x):
+    """What a row of numbers is held as (64 bits): e4m3 times the smallest power of two that keeps it within 448."""
+    x = x.double()
+    top = x.abs().amax(-1, keepdim=True)
+    e = torch.full_like(top, -126.0)
+    for k in range(-126, 129):  # (the smallest such power, by trying)
+        e = torch.where((e == -126) & (top > 448.0 * 2.0 ** -126) & (top <= 448.0 * 2.0 ** k) & (top > 448.0 * 2.0 ** (k - 1)),
+                        torch.full_like(e, float(k)), e)
+    y = x * torch.exp2(-e)
+    # e4m3: three bits of fraction, magnitudes below 2^-6 in steps of 2^-9, ties to even
+    step = torch.exp2(torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -6))) - 3)
+    return torch.round(y / step) * step * torch.exp2(e), e.squeeze(-1)
+
+
+@pytest.mark.parametrize("dh", [32, 96, 128])
+def test_rows_are_held_as_the_format_says(dh):
+    x = torch.randn(300, dh, generator=_gen(1)) * torch.exp2(torch.randint(-60, 60, (300, 1), generator=_gen(2)).float())
+    x[3], x[4, 1:] = 0.0, 0.0
+    x[5, 0] = 1.75 * 2.0 ** 9  # the largest magnitude is exactly at a border, and just beyond it
+    x[5, 1:] = 1.0
+    x[6] = x[5]
+    x[6, 0] = math.nextafter(1.75 * 2.0 ** 9, math.inf) * (1 + 2.0 ** -23)
+    x[7] = x[7] / x[7].abs().max() * 3.3e38
+    x[8] = x[8] / x[8].abs().max() * 2.0 ** -140
+    codes, byte = Q.quantize_rows(x)
+    want, e = held(x)
+    assert torch.equal(byte.double() - 127, e)
+    got = codes.view(torch.float8_e4m3fn).double() * torch.exp2(byte.double() - 127).unsqueeze(-1)
+    assert torch.equal(got, want)
+    # half a step: 2^-4 of a number's size, or 2^-10 of the codes' unit below 2^-6 of it
+    assert ((got - x.double()).abs() <= torch.maximum(2.0 ** -4 * x.double().abs(), torch.exp2(e - 10).unsqueeze(-1))).all()
+
+
+def test_rows_with_what_is_no_number_read_as_nan():
+    x = torch.randn(4, 64, generator=_gen(1))
+    x[1, 5], x[2, 0] = float("nan"), -float("inf")
+    kv = QuantizedPages.empty(2, 1, 16, 64, "cpu")
+    Q.store_rows(kv, x[:, None], x.flip(0)[:, None], torch.tensor([0, 17, 18, 3]))
+    k, v = Q.read_rows(kv, torch.tensor([0, 1]))
+    k, v = k.reshape(32, 64), v.reshape(32, 64)
+    assert torch.isnan(k[[17, 18]]).all() and not torch.isnan(k[[0, 3]]).any()
+    assert torch.isnan(v[[17, 18]]).all() and not torch.isnan(v[[0, 3]]).any()
+
+
+@pytest.mark.parametrize("dh", Q.HEAD_DIMS)
+def test_places_are_a_permutation_and_the_layout_that_the_lanes_take(dh):
+    k, v = Q.places(dh)
+    for at in (k, v):
+        assert sorted(at.flatten().tolist()) == list(range(16 * dh))
+    for piece in range(0, dh, 64):
+        u = 16 if dh - piece >= 64 else 8
+        for lane in (0, 5, 17, 40, 63):
+            r, g = lane % 16, lane // 16
+            assert [int(k[r, piece + u * g + i]) for i in range(u)] == [piece * 16 + lane * u + i for i in range(u)]
+            assert [int(v[4 * g + i % 4, piece + 16 * (i // 4) + r]) for i in range(u)] == [piece * 16 + lane * u + i for i in range(u)]
+
+
+def test_refusals():
+    for hq, hk, dh, ps in ((4, 2, 48, 16), (4, 2, 64, 24), (4, 2, 64, 8), (5, 2, 64, 16), (66, 2, 64, 16)):
+        with pytest.raises(ValueError, match="8 bits"):
+            Q.check_sizes(hq, hk, dh, ps)
+    with pytest.raises(ValueError, match="float8_e4m3"):
+        Q.check_kv_dtype("int4")
+    kv = QuantizedPages.empty(3, 2, 16, 64, "cpu")
+    assert tuple(kv.shape) == (3, 2, 2, 16, 64)
+    with pytest.raises(ValueError, match="uint8"):
+        QuantizedPages(kv.codes.float(), kv.scales)
+    with pytest.raises(ValueError, match="uint8"):
+        QuantizedPages(kv.codes, kv.scales[:1])
+    with pytest.raises(ValueError, match="contiguous"):
+        QuantizedPages(kv.codes.transpose(0, 1).contiguous().transpose(0, 1), kv.scales)
+
+
+# ------------------------------------------------------------------------------------------------ cases
+class Case:
+    """A step over pages in 8 bits: ``segs``: (tokens in the step, tokens of the request behind it)."""
+
+    def __init__(self, segs, hq, hk, dh, ps, rule=("all",), seed=0, device=DEV, single=False):
+        g = _gen(seed)
+        self.segs, self.hq, self.hk, self.dh, self.ps, self.rule = segs, hq, hk, dh, ps, rule
+        R = len(segs)
+        pages = [-(-t // ps) for _, t in segs]
+        width = max(pages)
+        P = sum(pages) + 2
+        ids = torch.randperm(P, generator=g).tolist()
+        table = torch.full((R, width), -1, dtype=torch.int32)
+        self.k = torch.full((P, hk, ps, dh), float("nan"), dtype=torch.float64)  # what is never written reads as NaN
+        self.v = self.k.clone()
+        kv = QuantizedPages.empty(P, hk, ps, dh, "cpu", poison=True)
+        pos, seg, slots = [], [], []
+        for i, (n, t) in enumerate(segs):
+            first = self.first(t - n)
+            for j in range(first // ps, pages[i]):  # (earlier pages were given back)
+                table[i, j] = ids.pop()
+            at = torch.arange(first // ps * ps, t)
+            slot = table[i, at // ps].long() * ps + at % ps
+            rows = [torch.randn(len(at), hk, dh, generator=g) * torch.exp2(torch.randint(-3, 4, (len(at), hk, 1), generator=g).float())
+                    for _ in range(2)]
+            Q.store_rows(kv, rows[0], rows[1], slot)
+            pos += range(t - n, t)
+            seg += [i] * n
+            slots += slot[-n:].tolist()
+        k, v = Q.read_rows(kv, torch.arange(P))
+        self.k, self.v = k.double(), v.double()
+        n = len(pos)
+        self.q = torch.randn(n, hq, dh, generator=g).bfloat16()
+        put = lambda x: torch.tensor(x, dtype=torch.int32, device=device)
+        self.cpu = (table, pos, seg)
+        self.kv = QuantizedPages(kv.codes.to(device), kv.scales.to(device))
+        self.table, self.positions, self.segment, self.slots = table.to(device), put(pos), put(seg), put(slots)
+        self.scale = dh ** -0.5
+        self.meta = GroupContext(block_table=self.table, slot_mapping=self.slots, width=width, retention=rule,
+                                 seg_lens=[a for a, _ in segs], seg_starts=[b - a for a, b in segs],
+                                 decode_bucket=decode_bucket(max(t for _, t in segs)) if single else None)
+
+    def first(self, pos):
+        if self.rule[0] == "chunk":
+            return pos // self.rule[1] * self.rule[1]
+        return max(0, pos - self.rule[1] + 1) if self.rule[0] == "window" else 0
+
+    def want(self, q=None):
+        """Attention in 64 bits, and how far bfloat16 may be off it: the probabilities times the rows' scales and the result
+        are rounded (half a step, 2^-8 each of the size); the scores are sums of dh products in float32, whose error moves a
+        probability by as much of its size, and so does the base-2 exponential's argument."""
+        table, pos, seg = self.cpu
+        q = (self.q if q is None else q).double()
+        out, tol = torch.empty_like(q), torch.empty_like(q)
+        G = self.hq // self.hk
+        for n, (p, i) in enumerate(zip(pos, seg)):
+            at = torch.arange(self.first(p), p + 1)
+            page = table[i, at // self.ps].long()
+            k, v = self.k[page, :, at % self.ps], self.v[page, :, at % self.ps]  # [T, hk, dh]
+            qi = q[n].view(self.hk, G, self.dh)
+            s = torch.einsum("hgd,thd->hgt", qi, k) * self.scale
+            size = (torch.einsum("hgd,thd->hgt", qi.abs(), k.abs()) * self.scale).amax(-1, keepdim=True)
+            w = torch.softmax(s, -1)
+            o = torch.einsum("hgt,thd->hgd", w, v)
+            a = torch.einsum("hgt,thd->hgd", w, v.abs())
+            out[n] = o.reshape(self.hq, self.dh)
+            off = 2 * (self.dh + 16) * 2.0 ** -24 * size + 2.0 ** -18 + len(at) * 2.0 ** -24
+            tol[n] = (2.0 ** -8 * (o.abs() + a) * (1 + 2.0 ** -8) + 2 * off * a).reshape(self.hq, self.dh)
+        return out.view(len(pos), -1), tol.view(len(pos), -1)
+
+    def run(self, ops, q=None):
+        return ops.paged_attention((self.q if q is None else q).to(self.table.device), self.kv, self.table, self.positions,
+                                   self.segment, self.rule, self.scale, self.meta)
+
+    def check(self, got, q=None):
+        want, tol = self.want(q)
+        far = (got.cpu().double() - want).abs()
+        assert (far <= tol).all(), f"off by {float((far / tol).max()):.3g} of what rounding allows"
+
+
+SEGS = {
+    "one token": [(1, 1)],
+    "second page": [(1, 17), (1, 16), (1, 33)],
+    "many": [(1, t) for t in (5, 700, 64, 333, 1025, 31, 32, 257)],
+    "few": [(4, 4), (3, 50), (2, 531), (1, 90)],
+    "portions": [(70, 70), (1, 300), (33, 215), (5, 12), (129, 400)],
+    "long": [(1, 9000)],
+}
+HEADS = [(4, 2, 64), (10, 2, 128), (16, 1, 32), (17, 1, 64), (3, 3, 96), (32, 1, 128), (4, 2, 256), (20, 1, 256)]
+
+
+@pytest.mark.parametrize("name", ["one token", "second page", "few"])
+@pytest.mark.parametrize("rule", [("all",), ("chunk", 24), ("window", 19)], ids=str)
+def test_plain_attention_over_codes(name, rule):
+    c = Case(SEGS[name], 4, 2, 64, 16, rule, seed=3, device="cpu")
+    c.check(c.run(ReferenceOps()))
+
+
+# ------------------------------------------------------------------------------------------------ on the GPU
+@gpu
+@pytest.mark.parametrize("dh", Q.HEAD_DIMS)
+def test_read_pages_gives_every_code_exactly(ops, dh):
+    g = _gen(dh)
+    for ps in (16, 48, 128):
+        kv = QuantizedPages(torch.randint(0, 256, (5, 3, 2, ps, dh), generator=g, dtype=torch.uint8),
+                            torch.randint(1, 248, (5, 3, 2, ps), generator=g, dtype=torch.uint8))
+        ids = torch.tensor([4, 0, -1, 4, 2, 5], dtype=torch.int32)
+        want = Q.read_pages(kv, ids)
+        got = ops.read_pages(QuantizedPages(kv.codes.to(DEV), kv.scales.to(DEV)), ids.to(DEV)).cpu()
+        # (numbers below bfloat16's smallest normal may be flushed)
+        same = (got == want) | (got.isnan() & want.isnan()) | ((want.float().abs() < 2.0 ** -126) & (got.float().abs() < 2.0 ** -126))
+        assert same.all() and got[[2, 5]].isnan().all()
+
+
+def _prepared(qkv, hq, hk, dh, pos, prep):
+    """Queries and keys in 64 bits (the angles are float32 products), values."""
+    x = qkv.double().view(len(pos), -1, dh)
+    h, v = x[:, : hq + hk].clone(), x[:, hq + hk:]
+    unit = lambda t: t / torch.sqrt((t * t).mean(-1, keepdim=True) + prep.norm_eps)
+    weights = torch.ones(hq + hk, dh, dtype=torch.float64)
+    if prep.norm_weight_q is not None:
+        weights[:hq], weights[hq:] = prep.norm_weight_q.double(), prep.norm_weight_k.double()
+    if prep.norm_eps is not None and prep.norm_first:
+        h = unit(h) * weights
+    r = prep.rotation
+    if r is not None:
+        ang = (torch.tensor(pos).float()[:, None] * r.inv_freq[None]).double()[:, None]
+        half = r.rotary_dim // 2
+        i = torch.arange(half)
+        a, b = (2 * i, 2 * i + 1) if r.pairing == "adjacent" else (i, i + half)
+        ha, hb = h[..., a], h[..., b]
+        h[..., a], h[..., b] = ha * ang.cos() - hb * ang.sin(), hb * ang.cos() + ha * ang.sin()
+    if prep.norm_eps is not None and not prep.norm_first:
+        h = unit(h) * weights
+    q = h[:, :hq]
+    if prep.query_scale is not None:
+        q = q * (1 + prep.query_scale[1] * torch.log1p(torch.floor((torch.tensor(pos).double() + 1) / prep.query_scale[0])))[:, None, None]
+    return q, h[:, hq:], v
+
+
+def _prep(kind, dh, device="cpu"):
+    g = _gen(dh)
+    rot = dh // 2 if kind in ("half part", "first") and dh >= 32 else dh
+    pairing = "half" if kind in ("half part", "half") else "adjacent"
+    freq = (10000.0 ** (-torch.arange(0, rot, 2).double() / rot)).float().to(device)
+    weights = {} if kind not in ("first", "weighted") else dict(norm_weight_q=(torch.rand(dh, generator=g) + 0.5).to(device),
+                                                               norm_weight_k=(torch.rand(dh, generator=g) + 0.5).to(device))
+    return QKPreparation(rotation=None if kind == "none" else Rotation(freq, pairing, rot),
+                         norm_eps=None if kind in ("none", "half") else 1e-5, norm_first=kind == "first",
+                         query_scale=(16.0, 0.3) if kind == "plain" else None, **weights)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["none", "plain", "half", "half part", "first", "weighted"])
+@pytest.mark.parametrize("hq,hk,dh", [(3, 1, 32), (4, 2, 64), (3, 3, 96), (10, 2, 128), (2, 1, 256)])
+@pytest.mark.parametrize("ps", [16, 48])
+def test_prepare_writes_rows_in_8_bits(ops, kind, hq, hk, dh, ps):
+    for n in (1, 5, 75):
+        g = _gen(n)
+        start = 7 if n > 1 else 100
+        pos = list(range(start, start + n))
+        qkv = (torch.randn(n, (hq + 2 * hk) * dh, generator=g) * 3).bfloat16()
+        qkv.view(n, -1, dh)[0, hq + hk] = 0.0  # a value of zeros
+        P = 9
+        kv = QuantizedPages.empty(P, hk, ps, dh, "cpu", poison=True)
+        order = torch.randperm(P, generator=g)
+        slots = torch.tensor([int(order[i // ps]) * ps + i % ps for i in range(3, 3 + n)], dtype=torch.int32)
+        if n > 4:
+            slots[2], slots[4] = -1, P * ps  # (rows without a place)
+        dev = QuantizedPages(kv.codes.to(DEV), kv.scales.to(DEV))
+        q = ops.qk_prepare_kv_write(qkv.to(DEV), hq, hk, dh, torch.tensor(pos, dtype=torch.int32, device=DEV),
+                                    _prep(kind, dh, DEV), dev, slots.to(DEV)).cpu().double()
+        prep = _prep(kind, dh)
+        wq, wk, wv = _prepared(qkv, hq, hk, dh, pos, prep)
+        # float32: two products and a sum a pair, sine and cosine to two units, the norm's sum and root: within 64 roundings
+        # of the pair's size (no pair is longer than the head's longest numbers)
+        slack = lambda x: 64 * 2.0 ** -24 * (x.abs() + x.abs().amax(-1, keepdim=True))
+        assert ((q - wq).abs() <= 2.0 ** -8 * wq.abs() + slack(wq)).all()
+        there = [i for i in range(n) if 0 <= slots[i] < P * ps]
+        s = slots[there].long()
+        k, v = (x.double().transpose(1, 2)[s // ps, s % ps] for x in Q.read_rows(QuantizedPages(dev.codes.cpu(), dev.scales.cpu()), torch.arange(P)))
+        for got, want, which in ((k, wk[there], 0), (v, wv[there], 1)):
+            full, e = held(want)
+            byte = dev.scales.cpu()[s // ps, :, which, s % ps].double() - 127
+            near = (torch.log2(want.abs().amax(-1) / 448) - e).abs() < 1e-5  # (at a border either scale is right)
+            assert ((byte == e) | near).all()
+            if which == 1:
+                assert torch.equal(got, full)  # (values are rounded from what was given)
+            assert ((got - want).abs() <= torch.maximum(2.0 ** -4 * want.abs(), torch.exp2(byte - 10).unsqueeze(-1)) + slack(want)).all()
+        # nothing else changed
+        untouched = torch.ones(P * ps, dtype=torch.bool)
+        untouched[s] = False
+        scales = dev.scales.cpu().permute(0, 3, 1, 2).reshape(P * ps, -1)
+        assert (scales[untouched] == Q.NAN_CODE).all()
+        rows = Q.read_rows(QuantizedPages(dev.codes.cpu(), torch.full_like(kv.scales, 127)), torch.arange(P))
+        for x in rows:
+            assert x.transpose(1, 2).reshape(P * ps, -1)[untouched].isnan().all()
+
+
+@gpu
+@pytest.mark.parametrize("hq,hk,dh", HEADS)
+@pytest.mark.parametrize("name", list(SEGS))
+def test_attention_over_codes(ops, hq, hk, dh, name):
+    c = Case(SEGS[name], hq, hk, dh, 16 if name != "many" else 48, seed=5)
+    c.check(c.run(ops))
+
+
+@gpu
+@pytest.mark.parametrize("rule", [("chunk", 256), ("chunk", 100), ("window", 300), ("window", 1), ("window", 33)], ids=str)
+@pytest.mark.parametrize("name", ["second page", "many", "few", "portions", "long"])
+def test_attention_over_codes_by_rule(ops, rule, name):
+    c = Case(SEGS[name], 10, 2, 128, 16, rule, seed=6)
+    c.check(c.run(ops))
+
+
+@gpu
+@pytest.mark.parametrize("ps", [16, 32, 48, 64, 256])
+@pytest.mark.parametrize("single", [False, True])
+def test_single_tokens_by_page_size_and_layout(ops, ps, single):
+    """A step of single tokens laid out for its own lengths, and for the next multiple of the recorded steps' bound."""
+    c = Case([(1, t) for t in (1, 15, 16, 17, 2000, 1024, 1025, 511)], 8, 4, 64, ps, seed=7, single=single)
+    c.check(c.run(ops))
+
+
+@gpu
+def test_scores_far_apart_and_alike(ops):
+    """Queries that make one key take all, and of zeros, where all keys weigh the same."""
+    c = Case([(1, 600), (40, 300), (2, 40)], 4, 2, 64, 16, seed=8)
+    q = c.q.clone()
+    q[0] *= 300
+    q[1:5] = 0
+    q[-1] *= 100
+    c.check(c.run(ops, q), q)
+
+
+@gpu
+def test_missing_pages_give_nan_to_their_queries_alone(ops):
+    for n in (1, 3, 40):
+        c = Case([(n, 200), (n, 200)], 4, 2, 64, 16, seed=9)
+        want, _ = c.want()
+        c.table[1, 5] = -1
+        got = c.run(ops).cpu()
+        assert not got[:n].isnan().any() and got[n:].isnan().all()
+        c.table[1, 5] = c.kv.shape[0]  # (a page that does not exist)
+        c.meta.meta.clear()
+        got = c.run(ops).cpu()
+        assert not got[:n].isnan().any() and got[n:].isnan().all()
+
+
+@gpu
+def test_refused_on_the_gpu(ops):
+    from jax_llm_examples_amd.ops.hip import KernelError
+
+    c = Case([(2, 40)], 4, 2, 64, 16)
+    q = c.q.to(DEV)
+    args = (c.table, c.positions, c.segment)
+    with pytest.raises(KernelError, match="score cap"):
+        ops.paged_attention(q, c.kv, *args, ("all",), 0.1, c.meta, cap=3.0)
+    with pytest.raises(KernelError, match="sinks"):
+        ops.paged_attention(q, c.kv, *args, ("all",), 0.1, c.meta, sink=torch.zeros(4, device=DEV))
+    with pytest.raises(KernelError, match="rules"):
+        ops.paged_attention(q, c.kv, *args, ("window_keep", 8, 2), 0.1, c.meta)
+    with pytest.raises(KernelError, match="positive"):
+        ops.paged_attention(q, c.kv, *args, ("all",), 0.0, c.meta)
+    with pytest.raises(KernelError, match="bfloat16"):
+        ops.paged_attention(q.float(), c.kv, *args, ("all",), 0.1, c.meta)
+    with pytest.raises(KernelError, match="pages of"):
+        ops.paged_attention(q.view(2, 2, 128), c.kv, *args, ("all",), 0.1, c.meta)
+    rows = torch.zeros(2, 8 * 64, dtype=torch.bfloat16, device=DEV)
+    pos = torch.zeros(2, dtype=torch.int32, device=DEV)
+    with pytest.raises(KernelError, match="multiple"):
+        ops.qk_prepare_kv_write(rows, 4, 2, 64, pos, QKPreparation(rotation=Rotation(torch.ones(12, device=DEV), "half", 24)), c.kv, pos)
+    with pytest.raises(KernelError, match="as they are"):
+        ops.qk_prepare_kv_write(rows, 4, 2, 64, pos, QKPreparation(rotation=Rotation(torch.ones(32, device=DEV), magnitude=2.0)), c.kv, pos)
+    with pytest.raises(KernelError, match="bfloat16"):
+        ops.qk_prepare_kv_write(rows.float(), 4, 2, 64, pos, QKPreparation(), c.kv, pos)
+    with pytest.raises(KernelError, match="must be on the GPU"):
+        ops.read_pages(QuantizedPages(c.kv.codes.cpu(), c.kv.scales.cpu()), pos)
+    with pytest.raises(KernelError, match="page ids"):
+        ops.read_pages(c.kv, pos.long())
