@@ -245,6 +245,7 @@ def main() -> int:
     ap.add_argument("--serve", default="", help="requests through the scheduler, e.g. 64x512+128@64 (requests x prompt "
                     "+ output tokens @ decode batch), comma-separated: tokens a second end to end")
     ap.add_argument("--preset", default="llama4-scout")
+    ap.add_argument("--kv-dtype", default=None, help="hold keys and values in 8 bits (float8_e4m3) instead of the run dtype")
     ap.add_argument("--no-prefill", action="store_true")
     ap.add_argument("--design-points", default="1@2048,8@2048,64@2048", help="decode steps of --designs: batch@context")
     ap.add_argument("--designs", default="", help="instead of the default workload: prefill and decode of the Rovidra, "
@@ -291,13 +292,21 @@ def main() -> int:
     need_tokens = (max([args.batch * (args.context + page)] + [b * (c + page) for b, c in points_at])
                    + max([args.prefill_tokens] + prefill_points) + 4 * page)
     ops = get_ops(dev)
-    cache = CacheManager(model.cache_needs(), page_size=page, num_pages=-(-need_tokens // page),
+    cache = CacheManager(model.cache_needs(args.kv_dtype), page_size=page, num_pages=-(-need_tokens // page),
                          max_requests=max(batches) + 1, dtype=model.dtype, device=dev)
     for g in cache.groups:  # stand-in keys and values for contexts that are not computed
         for t in g.tensors.values():
-            step = max(1, (1 << 28) // max(1, t[0].numel()))
-            for o in range(0, t.shape[0], step):
-                t[o: o + step].normal_(0.0, 0.5)
+            held = args.kv_dtype is not None  # (in 8 bits: the same numbers, as codes times 2^-8)
+            codes = t.codes if held else t
+            step = max(1, (1 << 28) // max(1, codes[0].numel()))
+            for o in range(0, codes.shape[0], step):
+                if held:
+                    x = torch.randn(codes[o: o + step].shape, device=dev, dtype=torch.bfloat16).mul_(128.0).clamp_(-448, 448)
+                    codes[o: o + step] = x.to(torch.float8_e4m3fn).view(torch.uint8)
+                else:
+                    codes[o: o + step].normal_(0.0, 0.5)
+            if held:
+                t.scales.fill_(127 - 8)
     runner = ModelRunner(model, cache, ops)
     sampler = Sampler(ops, dev)
     gen = torch.Generator().manual_seed(0)
@@ -393,7 +402,7 @@ def main() -> int:
         nreq, plen, olen = int(reqs_s), int(plen_s), int(olen_s)
         dbs = int(dbs_s) if dbs_s else min(nreq, 64)
         eng = Engine(model, cache_tokens=dbs * (plen + olen + 4 * page), decode_batch_size=dbs, page_size=page,
-                     max_num_batched_tokens=2048, max_seq_len=plen + olen + 8)
+                     max_num_batched_tokens=2048, max_seq_len=plen + olen + 8, kv_dtype=args.kv_dtype)
         prompts = [torch.randint(0, V, (plen,), generator=gen).tolist() for _ in range(nreq)]
         # (every other request samples with a temperature; none ends early)
         sp = [SamplingParams(max_decode_length=olen, sample_temp=0.0 if i % 2 == 0 else 0.8, seed=i, ignore_eos=True)
@@ -429,6 +438,7 @@ def main() -> int:
             "attention_chunk": cfg.attention_chunk_size, "global_batch": args.batch, "seq_len": args.context,
             "prefill_tokens": args.prefill_tokens, "page_size": page, "parallelism": "single-gpu",
             "mean_distinct_experts": round(mean_experts, 2),
+            **({} if args.kv_dtype is None else {"kv_dtype": args.kv_dtype}),
         },
         "prefill": prefill,
         "roofline": {"bound": "hbm", "achieved": round(achieved, 1), "peak": PEAK_HBM_GBS, "unit": "GB/s",

@@ -13,7 +13,8 @@ Runs of the model's order with the same ``(kv heads, head size, retention)``
 (and the same further per-token tensors, if any) form a *group*: they share page
 ids and one block table per request, and each has a tensor ``[num_pages, 2,
 kv_heads, page_size, head_dim]`` of its own (and ``[num_pages, page_size,
-*shape]`` for every further per-token tensor it declares).  Every group has a
+*shape]`` for every further per-token tensor it declares); a group whose keys and values are held in 8 bits has
+:class:`~..ops.quantized.QuantizedPages` in that tensor's place.  Every group has a
 pool of its own size: a group whose retention rule lets go of old tokens never
 holds more than a chunk (or window) plus one step's portion per request, so it
 needs far fewer pages than a group that keeps everything (:func:`pool_sizes`).
@@ -21,10 +22,12 @@ needs far fewer pages than a group that keeps everything (:func:`pool_sizes`).
 from __future__ import annotations
 
 import dataclasses
+import math
 from typing import Optional
 
 import torch
 
+from ..ops.quantized import QuantizedPages, bytes_per_row
 from ..parts.base import CacheNeed, first_needed_position, kept_prefix, retention_kind
 from .pages import OutOfPages, OutOfSlots, PagePool, SlotPool
 
@@ -37,22 +40,17 @@ class CacheGroup:
     retention: tuple
     cache_ids: list[int]
     pool: PagePool
-    tensors: dict[int, torch.Tensor]  # per run: [pages, 2, kv_heads, page_size, head_dim]
+    tensors: dict[int, torch.Tensor]  # per run: [pages, 2, kv_heads, page_size, head_dim], or QuantizedPages
     paged: tuple = ()  # further per-token tensors: (name, shape) pairs
     pages: dict[int, dict[str, torch.Tensor]] = dataclasses.field(default_factory=dict)  # per run, by name
     itemsize: int = 2
+    kv_dtype: Optional[str] = None  # keys and values in 8 bits (``None``: in the run dtype)
 
     def bytes_per_token(self, itemsize: int | None = None) -> int:
         """Bytes one token takes in this group, over all its runs."""
         if itemsize is None:
             itemsize = self.itemsize
-        per_run = 2 * self.kv_heads * self.head_dim
-        for _, shape in self.paged:
-            n = 1
-            for d in shape:
-                n *= d
-            per_run += n
-        return len(self.cache_ids) * per_run * itemsize
+        return len(self.cache_ids) * row_bytes((self.kv_heads, self.head_dim, self.kv_dtype), self.paged, itemsize)
 
 
 @dataclasses.dataclass
@@ -90,9 +88,18 @@ def group_key(need: CacheNeed):
     """Runs whose needs give the same key share page ids and block tables; ``None``: no pages."""
     if need.kv is None and not need.paged:
         return None
-    kv = (0, 0) if need.kv is None else (int(need.kv[0]), int(need.kv[1]))
+    kv = (0, 0, None) if need.kv is None else (int(need.kv[0]), int(need.kv[1]), need.kv_dtype)
     paged = tuple((str(n), tuple(int(d) for d in shape)) for n, shape in need.paged)
     return (kv, paged, tuple(need.retention))
+
+
+def row_bytes(kv: tuple, paged: tuple, itemsize: int) -> int:
+    """Bytes one token takes in one run's pages: ``kv``: (kv heads, head size, what they are held in)."""
+    heads, head_dim, held = kv
+    n = 2 * heads * (head_dim * itemsize if held is None else bytes_per_row(head_dim))
+    for _, shape in paged:
+        n += math.prod(shape) * itemsize
+    return n
 
 
 def plan_groups(needs: dict[int, CacheNeed]) -> list[tuple[tuple, list[int]]]:
@@ -133,13 +140,7 @@ def pool_sizes(needs: dict[int, CacheNeed], *, page_size: int, itemsize: int, ma
     for (kv, paged, retention), cids in groups:
         held = tokens_held_at_most(retention, max_step_tokens, max_seq_len)
         caps.append(None if held is None else max_requests * (-(-held // page_size) + 1))
-        per = 2 * kv[0] * kv[1]
-        for _, shape in paged:
-            n = 1
-            for d in shape:
-                n *= d
-            per += n
-        page_bytes.append(len(cids) * per * page_size * itemsize)
+        page_bytes.append(len(cids) * row_bytes(kv, paged, itemsize) * page_size)
 
     def sizes(pages_unbounded: int) -> list[int]:
         return [pages_unbounded if c is None else min(c, pages_unbounded) for c in caps]
@@ -200,11 +201,12 @@ class CacheManager:
         self._lives = 0  # requests added so far
         item = torch.empty((), dtype=dtype).element_size()
         for key, cids in plan_groups(needs):
-            (hk, dh), paged, retention = key
+            (hk, dh, held), paged, retention = key
             retention_kind(retention)  # (an unknown rule is an error here, not at the first page given back)
             i = len(self.groups)
             n = num_pages[i] if isinstance(num_pages, dict) else num_pages
-            g = CacheGroup(i, hk, dh, retention, list(cids), PagePool(n), {}, paged=paged, itemsize=item)
+            g = CacheGroup(i, hk, dh, retention, list(cids), PagePool(n), {}, paged=paged, itemsize=item,
+                           kv_dtype=held)
             self.groups.append(g)
             for cid in cids:
                 self.group_of[cid] = i
@@ -233,7 +235,10 @@ class CacheManager:
         fill = float("nan") if poison else 0.0
         for g in self.groups:
             for cid in g.cache_ids:
-                if g.kv_heads:
+                if g.kv_heads and g.kv_dtype is not None:
+                    g.tensors[cid] = QuantizedPages.empty(g.pool.num_pages, g.kv_heads, page_size, g.head_dim, self.device,
+                                                          poison=poison)
+                elif g.kv_heads:
                     g.tensors[cid] = torch.full(
                         (g.pool.num_pages, 2, g.kv_heads, page_size, g.head_dim), fill, dtype=dtype, device=self.device
                     )
@@ -382,7 +387,10 @@ class CacheManager:
         if self.poison and pages:
             idx = torch.tensor(pages, dtype=torch.long, device=self.device)
             for t in g.tensors.values():
-                t.index_fill_(0, idx, float("nan"))
+                if isinstance(t, QuantizedPages):
+                    t.poison_(idx)
+                else:
+                    t.index_fill_(0, idx, float("nan"))
             for named in g.pages.values():
                 for t in named.values():
                     t.index_fill_(0, idx, float("nan"))

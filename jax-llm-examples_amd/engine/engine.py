@@ -13,6 +13,7 @@ from typing import Optional, Sequence
 import torch
 
 from ..cache.manager import CacheManager, pool_sizes
+from ..ops.quantized import check_page_size
 from ..sampling.params import SamplingParams
 from ..sampling.sampler import Sampler
 from .batch import StepEntry
@@ -27,7 +28,7 @@ class Engine:
     def __init__(self, model, *, cache_tokens: Optional[int] = None, kv_memory_fraction: Optional[float] = None,
                  page_size: int = 16, decode_batch_size: int = 64, max_num_batched_tokens: int = 2048,
                  max_seq_len: Optional[int] = None, keep_free_pages: int = 0, reference_ops: bool = False,
-                 poison: bool = False, decode_graphs: Optional[bool] = None) -> None:
+                 poison: bool = False, decode_graphs: Optional[bool] = None, kv_dtype: Optional[str] = None) -> None:
         """The page pools are sized either by ``cache_tokens`` (tokens that a layer group which keeps
         every token can hold) or by ``kv_memory_fraction`` (that part of the device memory free now,
         after the weights).  With neither: ``decode_batch_size * max_seq_len`` tokens if ``max_seq_len``
@@ -35,6 +36,8 @@ class Engine:
         lets go of old tokens (chunked attention) get only what ``decode_batch_size`` requests can
         hold of them.  ``max_seq_len``: a request ends with reason ``"length"`` when prompt and
         output reach it; default: the configuration's ``max_position_embeddings``, if it has one.
+        ``kv_dtype``: ``"float8_e4m3"`` holds the attention layers' keys and values in 8 bits, each row with a power of two
+        of its own (about half the bytes of bfloat16; ``ValueError`` where a layer cannot have it so).
         ``decode_graphs``: replay steps of single tokens as recorded HIP graphs (default: on a GPU)."""
         self.model = model
         self.max_num_batched_tokens = max_num_batched_tokens
@@ -47,7 +50,9 @@ class Engine:
         elif limit is not None and max_seq_len > limit:
             raise ValueError(f"max_seq_len {max_seq_len} is beyond the model's max_position_embeddings {limit}")
         self.max_seq_len = max_seq_len
-        needs = model.cache_needs()
+        needs = model.cache_needs(kv_dtype)
+        if kv_dtype is not None:
+            check_page_size(page_size)
         item = torch.empty((), dtype=model.dtype).element_size()
         memory = None
         if kv_memory_fraction is not None:

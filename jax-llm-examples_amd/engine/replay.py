@@ -23,24 +23,25 @@ import torch
 
 from ..cache.manager import CacheManager
 from ..config.registry import architecture_name, get_architecture, read_config_json
+from ..ops.quantized import KV_DTYPES
 from .batch import StepEntry
 from .loading import get_ops, load_model, parse_dtype
 from .runner import ModelRunner
 
 def make_runner(model_dir: str, dtype, max_tokens: int, device: str = "cuda:0", page_size: int = 16,
                 max_requests: int = 8, reference_ops: bool = False, poison: bool = False,
-                decode_graphs=None) -> ModelRunner:
+                decode_graphs=None, kv_dtype=None) -> ModelRunner:
     """``max_tokens``: the most tokens live requests hold at any time, each request's count rounded
     up to a multiple of 64; every group's pool is made for that many (plus a page per request, for
     counts that are rounded to pages here), so pages are used again.  ``max_requests``: requests
-    that may be live at once."""
+    that may be live at once.  ``kv_dtype``: see :class:`~.engine.Engine`."""
     dtype = parse_dtype(dtype)
     arch = get_architecture(architecture_name(read_config_json(model_dir)))
     ops = get_ops(device, reference_ops=reference_ops, kernel_sources=getattr(arch, "kernel_sources", None))
     model = load_model(model_dir, dtype, device)
     rounded = -(-max_tokens // 64) * 64
     num_pages = -(-rounded // page_size) + max_requests
-    cache = CacheManager(model.cache_needs(), page_size=page_size, num_pages=num_pages,
+    cache = CacheManager(model.cache_needs(kv_dtype), page_size=page_size, num_pages=num_pages,
                          max_requests=max_requests, dtype=dtype, device=device, poison=poison,
                          run_states=model.run_state_needs())
     return ModelRunner(model, cache, ops, decode_graphs=decode_graphs)
@@ -80,11 +81,13 @@ def main(argv=None) -> int:
     ap.add_argument("--poison", action="store_true",
                     help="fill the page pools with NaN, and every page again when it is given back: a page that is "
                          "read without having been written by its present holder then shows in the logits")
+    ap.add_argument("--kv-dtype", choices=KV_DTYPES, help="hold keys and values in 8 bits instead of the run dtype")
     ap.add_argument("--no-decode-graphs", action="store_true",
                     help="run steps of single tokens launch by launch instead of replaying recorded HIP graphs")
     args = ap.parse_args(argv)
     runner = make_runner(args.model, args.dtype, args.max_tokens, args.device, args.page_size, args.max_requests,
-                         poison=args.poison, decode_graphs=False if args.no_decode_graphs else None)
+                         poison=args.poison, decode_graphs=False if args.no_decode_graphs else None,
+                         kv_dtype=args.kv_dtype)
     replay(runner, sys.stdin, args.out)
     return 0
 

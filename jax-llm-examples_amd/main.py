@@ -18,6 +18,8 @@ import time
 
 import torch
 
+from .ops.quantized import KV_DTYPES
+
 
 def _parse_prompts(args, vocab: int) -> list:
     prompts = []
@@ -61,6 +63,8 @@ def main(argv=None) -> int:
     ap.add_argument("--num-pages", type=int, help="the same in pages of --page-size tokens")
     ap.add_argument("--kv-memory-fraction", type=float,
                     help="size the page pools to this part of the device memory that is free after the weights")
+    ap.add_argument("--kv-dtype", choices=KV_DTYPES,
+                    help="hold the attention layers' keys and values in 8 bits (default: in the run dtype)")
     ap.add_argument("--no-decode-graphs", action="store_true",
                     help="run steps of single tokens launch by launch instead of replaying recorded HIP graphs")
     ap.add_argument("--profile", metavar="DIR",
@@ -107,7 +111,7 @@ def main(argv=None) -> int:
                                   or args.decode_batch_size * max_seq_len)
     engine = Engine(model, page_size=args.page_size, decode_batch_size=args.decode_batch_size,
                     max_num_batched_tokens=args.max_num_batched_tokens, max_seq_len=max_seq_len,
-                    decode_graphs=False if args.no_decode_graphs else None, **sizing)
+                    decode_graphs=False if args.no_decode_graphs else None, kv_dtype=args.kv_dtype, **sizing)
     eos = tuple(int(t) for t in args.eos_tokens.split(",") if t)
     params = [SamplingParams(sample_temp=args.sample_temp, sample_topk=args.sample_topk,
                              seed=args.sample_seed + i, max_decode_length=args.max_decode_length, eos_tokens=eos)

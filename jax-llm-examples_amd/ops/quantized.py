@@ -28,12 +28,16 @@ def check_kv_dtype(kv_dtype) -> None:
                          f"not in {kv_dtype!r}")
 
 
+def check_page_size(page_size: int) -> None:
+    if page_size < 16 or page_size % 16:
+        raise ValueError(f"a cache in 8 bits takes pages of a multiple of 16 tokens, not {page_size}")
+
+
 def check_sizes(num_heads: int, num_kv_heads: int, head_dim: int, page_size: int) -> None:
     """Raises ``ValueError`` for heads or pages that a cache in 8 bits does not take."""
     if head_dim not in HEAD_DIMS:
         raise ValueError(f"a cache in 8 bits takes heads of {', '.join(map(str, HEAD_DIMS))} elements, not {head_dim}")
-    if page_size < 16 or page_size % 16:
-        raise ValueError(f"a cache in 8 bits takes pages of a multiple of 16 tokens, not {page_size}")
+    check_page_size(page_size)
     if num_kv_heads < 1 or num_heads % num_kv_heads or num_heads // num_kv_heads > MOST_GROUPED:
         raise ValueError(f"a cache in 8 bits takes up to {MOST_GROUPED} query heads on each kv head, not {num_heads} on "
                          f"{num_kv_heads}")

@@ -44,6 +44,7 @@ import math
 
 import torch
 
+from ..ops.quantized import HEAD_DIMS, MOST_GROUPED
 from .base import CacheNeed, Mixer, ParamSpec, QKPreparation, build_position, first_needed_position, register_mixer
 
 
@@ -229,6 +230,20 @@ class Attention(Mixer):
             return CacheNeed(kv=(self.num_kv_heads, self.page_dim), retention=self.retention,
                              state_shape=(2, self.conv_taps - 1, self.channels), state_dtype=self.state_dtype)
         return CacheNeed(kv=(self.num_kv_heads, self.page_dim), retention=self.retention)
+
+    def check_kv_dtype(self, kv_dtype: str) -> None:
+        """The plain path takes a cache in 8 bits: q, k and v from one projection, a norm over the head or none, any rotation
+        of whole pairs, keys read under the rules all, chunk and window."""
+        if self.general or self.spanned or self.convolved:
+            raise ValueError(f"attention with a projection bias, a convolution, a norm over the projection, score maps, sinks, "
+                             f"gates or distance terms keeps its keys and values in the run dtype, not in {kv_dtype}")
+        if self.head_dim not in HEAD_DIMS or self.num_heads // self.num_kv_heads > MOST_GROUPED:
+            raise ValueError(f"keys and values are held in {kv_dtype} for heads of {', '.join(map(str, HEAD_DIMS))} with up to "
+                             f"{MOST_GROUPED} query heads on a kv head, not {self.head_dim} with "
+                             f"{self.num_heads // self.num_kv_heads}")
+        rot = self.position.rotation()
+        if rot is not None and rot.pairing == "half" and (int(rot.rotary_dim) or self.head_dim) % 16:
+            raise ValueError(f"with {kv_dtype} the part of a head that is rotated in half-split pairs is a multiple of 16")
 
     graph_safe = True
 

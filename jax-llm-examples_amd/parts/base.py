@@ -100,6 +100,9 @@ class CacheNeed:
     # (``CacheView.pages[name]``).  ``kv`` is the layout the attention kernels read (keys ``[page_size,
     # head_dim]`` and values transposed in one tensor).
     paged: tuple = ()
+    # What the keys and values of ``kv`` are held in: ``None`` for the run dtype, or a name of
+    # ``ops.quantized.KV_DTYPES`` (whoever runs the model asks for it: ``DecoderModel.cache_needs``).
+    kv_dtype: Optional[str] = None
     # Further fixed-size state per request, by name: a tuple of ``(name, shape, dtype)``; each becomes a tensor
     # ``[slots, *shape]``, cleared when a request is admitted, that the mixer finds in ``CacheView.states[name]``
     # (a mixer that keeps a recurrent memory in float32 beside a convolution's last rows in the run dtype; a mixer
@@ -177,6 +180,10 @@ class Mixer(Part):
 
     def cache_need(self) -> CacheNeed:
         return CacheNeed()
+
+    def check_kv_dtype(self, kv_dtype: str) -> None:
+        """Raises ``ValueError`` if this mixer's keys and values (:attr:`CacheNeed.kv`) cannot be held in ``kv_dtype``."""
+        raise ValueError(f"{type(self).__name__} keeps its keys and values in the run dtype, not in {kv_dtype}")
 
     def mixing_flops(self, start: int, count: int) -> float:
         """Floating-point operations of moving information between positions (beyond the matrix

@@ -3,10 +3,13 @@ final norm and output head (``llama4/llama4_jax/model.py:1186-1210``), each a pa
 its :class:`~..config.specs.PartSpec`.  It is built from a :class:`~..config.specs.ModelPlan` alone."""
 from __future__ import annotations
 
+import dataclasses
+
 import torch
 
 from ..cache.manager import CacheView
 from ..config.specs import ModelPlan
+from ..ops.quantized import check_kv_dtype
 from .residual import build_residual
 from ..config.specs import part
 from . import embedding as _ends  # noqa: F401  (registers the built-in embedding and head)
@@ -69,13 +72,31 @@ class DecoderModel:
         return n
 
     # ------------------------------------------------------------------ cache
-    def cache_needs(self) -> dict[int, CacheNeed]:
+    def cache_needs(self, kv_dtype=None) -> dict[int, CacheNeed]:
+        """What every cache of the run order has to hold.  ``kv_dtype``: what the keys and values of the attention layers
+        are held in instead of the run dtype (a name of ``ops.quantized.KV_DTYPES``); further per-token tensors and
+        state stay as they are.  Raises ``ValueError`` if a layer of the model cannot have it so, or none would."""
+        check_kv_dtype(kv_dtype)
         needs: dict[int, CacheNeed] = {}
         for e in self.plan.order:
             need = self.blocks[e.layer].mixer.cache_need()
             if e.cache in needs and needs[e.cache] != need:
                 raise ValueError(f"runs that share cache {e.cache} need different things: {needs[e.cache]} vs {need}")
             needs[e.cache] = need
+        if kv_dtype is not None:
+            held = {cid for cid, need in needs.items() if need.kv is not None}
+            if not held:
+                raise ValueError(f"no layer of this model keeps keys and values that could be held in {kv_dtype}")
+            if self.dtype != torch.bfloat16:
+                raise ValueError(f"keys and values are held in {kv_dtype} beside a run dtype of bfloat16, not {self.dtype}")
+            for e in self.plan.order:
+                if e.cache in held:
+                    try:
+                        self.blocks[e.layer].mixer.check_kv_dtype(kv_dtype)
+                    except ValueError as err:
+                        raise ValueError(f"layer {e.layer}: {err}") from None
+            needs = {cid: dataclasses.replace(need, kv_dtype=kv_dtype) if cid in held else need
+                     for cid, need in needs.items()}
         return needs
 
     def run_state_needs(self) -> dict[int, dict]:

@@ -379,3 +379,145 @@ def test_refused_on_the_gpu(ops):
         ops.read_pages(QuantizedPages(c.kv.codes.cpu(), c.kv.scales.cpu()), pos)
     with pytest.raises(KernelError, match="page ids"):
         ops.read_pages(c.kv, pos.long())
+
+
+# ------------------------------------------------------------------------------------------------ the engine
+def _engine(folder, device, kv_dtype="float8_e4m3", **kw):
+    from jax_llm_examples_amd import Engine, load_model
+
+    cpu = device == "cpu"
+    return Engine(load_model(folder, "bfloat16", device), cache_tokens=1024, decode_batch_size=4,
+                  **{"max_num_batched_tokens": 32, "kv_dtype": kv_dtype, "reference_ops": cpu, **kw})
+
+
+def _prompts(vocab, lengths=(7, 40, 19)):
+    return [torch.randint(0, vocab, (n,), generator=_gen(n)).tolist() for n in lengths]
+
+
+def test_engine_keeps_its_cache_in_8_bits(model_dirs_bf16):
+    """Tiny configuration B (heads of 32): pages of codes, their bytes, poisoned pages that nobody reads, and logits whose
+    distance from the bfloat16 cache's is what 8 bits cost."""
+    e = _engine(model_dirs_bf16["B"], "cpu", poison=True)
+    for g in e.cache.groups:
+        assert all(isinstance(t, QuantizedPages) and tuple(t.shape[1:]) == (2, 3, 16, 32) for t in g.tensors.values())
+        assert g.bytes_per_token() == len(g.cache_ids) * 2 * 3 * 33
+        assert sum(t.codes.numel() + t.scales.numel() for t in g.tensors.values()) == g.bytes_per_token() * 16 * g.pool.num_pages
+    plain = _engine(model_dirs_bf16["B"], "cpu", kv_dtype=None)
+    prompts = _prompts(1000)
+    _, a, ids = e.prefill(prompts)
+    _, b, ids_b = plain.prefill(prompts)
+    for step in range(20):  # (past the chunk of 48 and several pages)
+        far = float((a - b).norm() / b.norm())
+        assert torch.isfinite(a).all() and far < 0.1, far
+        a, b = e.decode_step([step] * 3, ids)[1], plain.decode_step([step] * 3, ids_b)[1]
+    e.release(ids)
+    e.cache.check()
+
+
+def test_engine_with_8_bits_gives_the_same_logits_however_prompts_are_cut(model_dirs_bf16):
+    got = []
+    for budget in (5, 64):
+        e = _engine(model_dirs_bf16["B"], "cpu", max_num_batched_tokens=budget, poison=True)
+        got.append(e.prefill(_prompts(1000))[1])
+    assert torch.allclose(got[0], got[1], rtol=1e-4, atol=1e-4)
+
+
+def test_pool_sizes_by_memory_hold_about_twice_the_tokens(model_dirs_bf16):
+    from jax_llm_examples_amd import load_model
+    from jax_llm_examples_amd.cache import plan_groups, pool_sizes
+
+    model = load_model(model_dirs_bf16["B"], "bfloat16", "cpu")
+    kw = dict(page_size=16, itemsize=2, max_requests=4, max_step_tokens=64, memory_bytes=1 << 20)
+    wide, narrow = pool_sizes(model.cache_needs(), **kw), pool_sizes(model.cache_needs("float8_e4m3"), **kw)
+    everything = [i for i, (key, _) in enumerate(plan_groups(model.cache_needs())) if key[2] == ("all",)]
+    assert len(everything) == 1 and narrow[everything[0]] > 1.9 * wide[everything[0]]
+
+
+def test_engines_that_refuse_8_bits(model_dirs, model_dirs_bf16, tmp_path):
+    from jax_llm_examples_amd import Engine, load_model
+
+    with pytest.raises(ValueError, match="heads of"):
+        _engine(model_dirs_bf16["A"], "cpu")  # (heads of 16)
+    with pytest.raises(ValueError, match="multiple of 16 tokens"):
+        _engine(model_dirs_bf16["B"], "cpu", page_size=8)
+    with pytest.raises(ValueError, match="int8"):
+        _engine(model_dirs_bf16["B"], "cpu", kv_dtype="int8")
+    with pytest.raises(ValueError, match="beside a run dtype of bfloat16"):
+        Engine(load_model(model_dirs["B"], "float32", "cpu"), cache_tokens=64, reference_ops=True, kv_dtype="float8_e4m3")
+
+
+def test_designs_whose_attention_keeps_its_run_dtype_refuse_8_bits():
+    import mazotar_configs
+    import rovidra_configs
+    from jax_llm_examples_amd.config import get_architecture
+    from jax_llm_examples_amd.engine import build_model
+
+    for configs, table, words in ((mazotar_configs, "MAZOTAR", "layer"), (rovidra_configs, "ROVIDRA", "no layer")):
+        top = next(iter(getattr(configs, table).values()))
+        top = {k: v for k, v in top.items() if k != "seed"}
+        arch = get_architecture(top["architecture"])
+        with pytest.raises(ValueError, match=words):
+            build_model(arch, arch.parse_config(top), "bfloat16", "cpu").cache_needs("float8_e4m3")
+
+
+@gpu
+@pytest.mark.parametrize("name", ["B", "F"])
+def test_engine_on_the_gpu_follows_the_plain_one(name, tmp_path):
+    """Portions, single tokens, recorded steps: logits of the kernels beside those of the plain operations, both with a cache
+    in 8 bits, over pages that are NaN until they are written."""
+    from tiny_configs import write_tiny
+
+    folder = write_tiny(name, str(tmp_path / name), torch.bfloat16)
+    e, p = _engine(folder, DEV, poison=True), _engine(folder, "cpu", poison=True)
+    prompts = _prompts(600, (7, 40, 90))
+    _, a, ids = e.prefill(prompts)
+    _, b, ids_p = p.prefill(prompts)
+    for step in range(12):
+        far = float((a.cpu() - b).norm() / b.norm())
+        assert far < 0.03, (step, far)  # (bfloat16 activations through a few layers: each rounding 2^-9 on average)
+        a, b = e.decode_step([step + 1] * 3, ids)[1], p.decode_step([step + 1] * 3, ids_p)[1]
+    assert e.runner.graphs.replays > 0
+
+
+@gpu
+def test_recorded_steps_over_8_bits_equal_unrecorded_ones_bit_for_bit(tmp_path):
+    from tiny_configs import write_tiny
+
+    folder = write_tiny("F", str(tmp_path / "F"), torch.bfloat16)
+    a, b = _engine(folder, DEV, poison=True), _engine(folder, DEV, decode_graphs=False)
+    prompts = _prompts(600, (7, 40, 90, 1))
+    _, la, ids = a.prefill(prompts)
+    _, lb, ids_b = b.prefill(prompts)
+    assert torch.equal(la, lb)
+    for step in range(30):
+        la, lb = a.decode_step([step] * 4, ids)[1], b.decode_step([step] * 4, ids_b)[1]
+        assert torch.equal(la, lb), step
+    assert a.runner.graphs.replays >= 28 and b.runner.graphs is None
+
+
+@gpu
+def test_a_layer_from_its_rows_writes_reads_and_attends(ops):
+    """The calls of a layer one after the other, as a step makes them: a portion, then single tokens, then a few at once,
+    each attending to what the steps before it wrote, against attention in 64 bits over the rows that the pages hold."""
+    hq, hk, dh, ps, P = 10, 2, 128, 16, 40
+    kv = QuantizedPages.empty(P, hk, ps, dh, DEV, poison=True)
+    prep = _prep("plain", dh, DEV)
+    table = torch.randperm(P, generator=_gen(1))[:20].to(torch.int32).view(1, -1)
+    done = 0
+    for n in (130, 1, 1, 4, 33, 1):
+        c = Case.__new__(Case)
+        c.segs, c.hq, c.hk, c.dh, c.ps, c.rule, c.scale = [(n, done + n)], hq, hk, dh, ps, ("chunk", 150), dh ** -0.5
+        pos = list(range(done, done + n))
+        put = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+        slots = put([int(table[0, p // ps]) * ps + p % ps for p in pos])
+        qkv = (torch.randn(n, (hq + 2 * hk) * dh, generator=_gen(n)) * 2).bfloat16().to(DEV)
+        meta = GroupContext(block_table=table.to(DEV), slot_mapping=slots, width=20, retention=c.rule, seg_lens=[n],
+                            seg_starts=[done], decode_bucket=decode_bucket(done + n) if n == 1 else None)
+        got = ops.attention_from_qkv(qkv, hq, hk, dh, put(pos), put([0] * n), prep, kv, True, slots, table.to(DEV), c.rule,
+                                     c.scale, meta)
+        done += n
+        k, v = Q.read_rows(QuantizedPages(kv.codes.cpu(), kv.scales.cpu()), torch.arange(P))
+        c.k, c.v, c.cpu = k.double(), v.double(), (table, pos, [0] * n)
+        # (the queries, as a step that writes nothing prepares them)
+        q = ops.qk_prepare_kv_write(qkv, hq, hk, dh, put(pos), prep, kv, torch.full_like(slots, -1)).cpu()
+        c.check(got, q)
