@@ -13,27 +13,43 @@
 // steps in registers or on their way.  What bounds it is memory: 2 * dh + 2 bytes a key and kv head.
 //
 // The wavefronts' (maximum, sum, unnormalised O^T) are merged in shared memory; with more than one range a (tile, kv head)
-// the blocks' results go through memory and a second kernel merges them in order.  Which ranges there are depends on the
-// position, the retention rule and `range` alone.
+// the blocks' results go through memory, and the block that takes the last ticket adds them up in the ranges' order.  Which
+// ranges there are depends on the position, the retention rule and `range` alone.
 #include "mfma_attention.h"
 #include "quantized.h"
 
 using namespace jle;
 
-__device__ __forceinline__ int first_key(int mode, int param, int pos) {
-  if (mode == 1) return (pos / param) * param;
-  if (mode == 2) return pos - param + 1 > 0 ? pos - param + 1 : 0;
-  return 0;
+// x / d for 0 <= x < 2^31 by a product: with floor(2^32 / d) (2^32 - 1 for one) the estimate is the quotient or one less.
+// (A division of two numbers that are only known when the kernel runs is tens of instructions, and a short launch waits for
+// every instruction that it meets for the first time.)
+struct Divisor {
+  uint32_t d, magic;
+};
+static Divisor divisor(int d) { return {(uint32_t)d, d == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (uint32_t)d)}; }
+__device__ __forceinline__ int over(int x, Divisor by) {
+  const uint32_t q = __umulhi((uint32_t)x, by.magic);
+  return (int)(q + ((uint32_t)x - q * by.d >= by.d));
 }
 
+// The first key that a query at `pos` reads: rules all (0), chunk (1), window (2).
+struct Rule {
+  int mode;
+  Divisor param;
+  __device__ __forceinline__ int first(int pos) const {
+    if (mode == 0) return 0;
+    if (mode == 1) return over(pos, param) * (int)param.d;
+    return max(pos - (int)param.d + 1, 0);
+  }
+};
+
 template <int DH>
-struct QuantizedStep {  // 32 keys of one kv head
+struct QuantizedStep {  // 32 keys of one kv head: two tiles of sixteen
   static constexpr int P = DH / 64;                // pieces of 64 elements
   static constexpr bool T = DH % 64 != 0;          // a last piece of 32
   u32x4 k[2][P > 0 ? P : 1], v[2][P > 0 ? P : 1];
   u32x2 kt[2], vt[2];
   uint32_t ks[2], vs[2];  // scale bytes: of the lane's key; of its four keys
-  int have;               // bit tt: the tile of sixteen keys exists
 };
 
 __device__ __forceinline__ uint32_t two_codes(uint32_t w, float scale, bool hi) {
@@ -45,47 +61,45 @@ __device__ __forceinline__ bf16x8 eight_codes(uint32_t a, uint32_t b, float scal
   return __builtin_bit_cast(bf16x8, r);
 }
 
+// Two floats written to / read from where all compute units see them at once: for what blocks on different dies hand each
+// other within a launch.
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+__device__ __forceinline__ void put_through(float* p, float a, float b) {
+  const f32x2 v = {a, b};
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f32x2 get_through(const float* p) {
+  return __builtin_bit_cast(f32x2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                                     __HIP_MEMORY_SCOPE_AGENT));
+}
+constexpr int kMostRanges = 128;  // of a (tile, kv head): their maxima and sums fit where the wavefronts' results lay
+
 template <int DH, int CT, int W>
 __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
     const bf16_t* __restrict__ q, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-    bf16_t* __restrict__ out, float* __restrict__ ws_ml, float* __restrict__ ws_o, const int* __restrict__ positions,
+    bf16_t* __restrict__ out, float* __restrict__ ws_ml, float* __restrict__ ws_o, int* __restrict__ tickets,
+    const int* __restrict__ positions,
     const int* __restrict__ token_segment, const int* __restrict__ block_table, int table_width, int num_pages,
-    const int* __restrict__ tiles, int ranges, int range, int ret_mode, int ret_param, float scale_log2, int Hq, int Hkv,
-    int ps, int max_cols) {
+    const int* __restrict__ tiles, int ranges, Divisor range, Rule rule, float scale_log2, int Hq, int Hkv, Divisor group,
+    Divisor page_tiles, int max_cols) {
   using Step = QuantizedStep<DH>;
   constexpr int P = Step::P, DT = DH / 16, KC = DH / 32, LD = DH + 4;
   extern __shared__ __attribute__((aligned(16))) float smem[];  // [W][max_cols][LD], then [W][max_cols][2]
   const int lane = threadIdx.x & 63, wave = wave_index();
   const int c16 = lane & 15, g = lane >> 4;
-  const int hk = blockIdx.x % Hkv;
-  const int rng = (blockIdx.x / Hkv) % ranges;
-  const int tile = blockIdx.x / (Hkv * ranges);
-  const int n0 = tiles[2 * tile], nt = tiles[2 * tile + 1];
+  const int hk = blockIdx.x, tile = blockIdx.y, rng = blockIdx.z;  // (ranges that few tiles have come last)
+  const int ps = 16 * (int)page_tiles.d, G = (int)group.d;
+  const int n0 = tiles != nullptr ? tiles[2 * tile] : tile, nt = tiles != nullptr ? tiles[2 * tile + 1] : 1;
   const int p_first = positions[n0], p_last = p_first + nt - 1;
-  const int first = first_key(ret_mode, ret_param, p_first);
-  const int r_abs = first / range + rng;
-  if (r_abs > p_last / range) return;  // (this tile has fewer ranges)
-  const int k_lo = max(first, r_abs * range), k_hi = min(p_last, r_abs * range + range - 1);
-  const int full_lo = max(k_lo, first_key(ret_mode, ret_param, p_last)), full_hi = min(k_hi, p_first);
-  const int G = Hq / Hkv, cols = nt * G;
+  const int first = rule.first(p_first);
+  const int r_first = over(first, range), r_abs = r_first + rng, mine = over(p_last, range) - r_first + 1;
+  if (rng >= mine) return;  // (this tile has fewer ranges)
+  const int k_lo = max(first, r_abs * (int)range.d), k_hi = min(p_last, r_abs * (int)range.d + (int)range.d - 1);
+  const int full_lo = max(k_lo, rule.first(p_last)), full_hi = min(k_hi, p_first);
+  const int cols = nt * G;
   const int* table = block_table + (size_t)token_segment[n0] * table_width;
 
-  int lo[CT], hi[CT];
-  bf16x8 qb[CT][KC];
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const int c = ct * 16 + c16;
-    const int t = c < cols ? c / G : 0, head = hk * G + (c < cols ? c - t * G : 0);
-    lo[ct] = max(k_lo, first_key(ret_mode, ret_param, p_first + t));
-    hi[ct] = min(k_hi, p_first + t);
-    const bf16_t* row = q + ((size_t)(n0 + t) * Hq + head) * DH;
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      qb[ct][2 * p] = *reinterpret_cast<const bf16x8*>(row + 64 * p + 16 * g);
-      qb[ct][2 * p + 1] = *reinterpret_cast<const bf16x8*>(row + 64 * p + 16 * g + 8);
-    }
-    if (Step::T) qb[ct][KC - 1] = *reinterpret_cast<const bf16x8*>(row + 64 * P + 8 * g);
-  }
   float m[CT], l[CT];
   f32x4 acc[CT][DT];
 #pragma unroll
@@ -96,35 +110,37 @@ __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
     for (int dt = 0; dt < DT; ++dt) acc[ct][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   bool bad = false;
+  int lo[CT], hi[CT];
+  bf16x8 qb[CT][KC];
 
-  auto load = [&](Step& s, int step) {
-    s.have = 0;
+  // The pages of a step are looked up, through the scalar path, two steps before their data is asked for: no load waits for
+  // the block table.  And every load is issued, whether its keys exist or not (then it reads page 0, and what it brings is
+  // masked or not used): the wait for one step's data then never includes the next one's.
+  struct Pages {
+    int id[2], off[2];  // per tile of sixteen keys: its page, the place of its first key there
+  };
+  auto look_up = [&](Pages& at, int step) {
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
       const int key0 = 32 * step + 16 * tt;
-      int page = -1, off = 0;
-      if (key0 <= k_hi && key0 + 15 >= k_lo) {
-        const int idx = key0 / ps;
-        off = key0 - idx * ps;
-        page = idx < table_width ? table[idx] : -1;
-        if (page < 0 || page >= num_pages) {
-          bad = true;  // (the tile is left out, and the result is NaN)
-          page = -1;
-        }
-      }
+      const int idx = over(key0 >> 4, page_tiles);
+      const bool there = (key0 <= k_hi) & (key0 + 15 >= k_lo) & (idx < table_width);
+      const int id = table[there ? idx : 0];  // (without a branch; a table is at least one page wide)
+      at.id[tt] = there ? id : -1;
+      at.off[tt] = key0 - idx * ps;
+    }
+  };
+  const uint32_t page_rows = (uint32_t)Hkv * 2 * ps;
+  auto load = [&](Step& s, const Pages& at, int step) {
 #pragma unroll
-      for (int p = 0; p < P; ++p) {
-        s.k[tt][p] = u32x4{0u, 0u, 0u, 0u};
-        s.v[tt][p] = u32x4{0u, 0u, 0u, 0u};
-      }
-      s.kt[tt] = s.vt[tt] = u32x2{0u, 0u};
-      s.ks[tt] = s.vs[tt] = 0u;
-      if (page < 0) continue;
-      s.have |= 1 << tt;
-      const size_t plane = ((size_t)page * Hkv + hk) * 2;
-      const uint8_t* kp = codes + (plane * ps + off) * DH;
-      const uint8_t* vp = kp + (size_t)ps * DH;
-      const uint8_t* sp = scales + plane * ps + off;
+    for (int tt = 0; tt < 2; ++tt) {
+      const int key0 = 32 * step + 16 * tt, page = at.id[tt];
+      const bool ok = (page >= 0) & (page < num_pages);
+      bad |= !ok & (key0 <= k_hi) & (key0 + 15 >= k_lo);  // (a page is missing: the result is NaN)
+      const uint64_t row = (uint64_t)(uint32_t)(ok ? page : 0) * page_rows + (uint32_t)(hk * 2 * ps + (ok ? at.off[tt] : 0));
+      const uint8_t* kp = codes + row * DH;
+      const uint8_t* vp = kp + ps * DH;
+      const uint8_t* sp = scales + row;
       s.ks[tt] = sp[c16];
       s.vs[tt] = *reinterpret_cast<const uint32_t*>(sp + ps + 4 * g);
 #pragma unroll
@@ -152,23 +168,27 @@ __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
         for (int ct = 0; ct < CT; ++ct) st[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qb[ct][c], st[ct][tt], 0, 0, 0);
       }
     }
-    const bool full = s.have == 3 && 32 * step >= full_lo && 32 * step + 31 <= full_hi;
-    uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+    const bool full = 32 * step >= full_lo && 32 * step + 31 <= full_hi;
     if (!full) {
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt) {
-        keep[tt] = 0u;
+        uint32_t keep = 0u;  // values and scales of keys outside the range may never have been written: they are read as zero
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = 32 * step + 16 * tt + 4 * g + i;
-          const bool there = (s.have >> tt & 1) != 0;
-          // values and scales of keys outside the range may never have been written: they are read as zero
-          if (there && key >= k_lo && key <= k_hi) keep[tt] |= 255u << (8 * i);
+          keep |= (key >= k_lo) & (key <= k_hi) ? 255u << (8 * i) : 0u;
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct)
-            if (!(there && key >= lo[ct] && key <= hi[ct])) st[ct][tt][i] = -INFINITY;
+          for (int ct = 0; ct < CT; ++ct) st[ct][tt][i] = (key >= lo[ct]) & (key <= hi[ct]) ? st[ct][tt][i] : -INFINITY;
         }
-        s.vs[tt] &= keep[tt];
+        s.vs[tt] &= keep;
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s.v[tt][p][j] &= keep;
+        if (Step::T) {
+          s.vt[tt][0] &= keep;
+          s.vt[tt][1] &= keep;
+        }
       }
     }
     float vf[8];
@@ -210,9 +230,8 @@ __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       const bool tail = Step::T && dt >= 4 * P;
-      const uint32_t w0 = (tail ? s.vt[0][dt & 1] : s.v[0][dt / 4][dt & 3]) & keep[0];
-      const uint32_t w1 = (tail ? s.vt[1][dt & 1] : s.v[1][dt / 4][dt & 3]) & keep[1];
-      const bf16x8 a = eight_codes(w0, w1, 1.0f);
+      const bf16x8 a = eight_codes(tail ? s.vt[0][dt & 1] : s.v[0][dt / 4][dt & 3],
+                                   tail ? s.vt[1][dt & 1] : s.v[1][dt / 4][dt & 3], 1.0f);
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) acc[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pb[ct], acc[ct][dt], 0, 0, 0);
     }
@@ -221,16 +240,39 @@ __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
   const int last = k_hi / 32;
   int step = k_lo / 32 + wave;
   Step a, b;
-  if (step <= last) load(a, step);
-  if (step + W <= last) load(b, step + W);
-  while (step <= last) {
+  Pages pa, pb;
+  look_up(pa, step);
+  look_up(pb, step + W);
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int c = ct * 16 + c16;
+    const int t = c < cols ? over(c, group) : 0, head = hk * G + (c < cols ? c - t * G : 0);
+    lo[ct] = max(k_lo, rule.first(p_first + t));
+    hi[ct] = min(k_hi, p_first + t);
+    const bf16_t* row = q + ((size_t)(n0 + t) * Hq + head) * DH;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      qb[ct][2 * p] = *reinterpret_cast<const bf16x8*>(row + 64 * p + 16 * g);
+      qb[ct][2 * p + 1] = *reinterpret_cast<const bf16x8*>(row + 64 * p + 16 * g + 8);
+    }
+    if (Step::T) qb[ct][KC - 1] = *reinterpret_cast<const bf16x8*>(row + 64 * P + 8 * g);
+  }
+  __builtin_amdgcn_sched_barrier(0);  // (the queries first, then one step's loads before the next one's: the waits count them)
+  load(a, pa, step);
+  __builtin_amdgcn_sched_barrier(0);
+  load(b, pb, step + W);
+  __builtin_amdgcn_sched_barrier(0);
+  look_up(pa, step + 2 * W);
+  look_up(pb, step + 3 * W);
+  for (; step <= last; step += 2 * W) {  // (no way through the loop leaves out a load)
     work(a, step);
-    if (step + 2 * W <= last) load(a, step + 2 * W);
-    step += W;
-    if (step > last) break;
-    work(b, step);
-    if (step + 2 * W <= last) load(b, step + 2 * W);
-    step += W;
+    load(a, pa, step + 2 * W);
+    __builtin_amdgcn_sched_barrier(0);
+    look_up(pa, step + 4 * W);
+    if (step + W <= last) work(b, step + W);
+    load(b, pb, step + 3 * W);
+    __builtin_amdgcn_sched_barrier(0);
+    look_up(pb, step + 5 * W);
   }
   bad = __any(bad);
 
@@ -250,6 +292,9 @@ __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
     }
   }
   __syncthreads();
+  // (column, four elements) items: a block's result, or its part of one
+  const size_t part0 = ((size_t)tile * Hkv + hk) * ranges;
+  const bool alone = mine == 1;
   for (int i = threadIdx.x; i < cols * (DH / 4); i += W * 64) {
     const int c = i / (DH / 4), d = 4 * (i - c * (DH / 4));
     float top = -INFINITY;
@@ -271,100 +316,109 @@ __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = fmaf(v[e], f, o[e]);
     }
-    const int t = c / G;
-    if (ranges == 1) {
+    if (alone) {
+      const int t = over(c, group);
       const float inv = nan ? __builtin_nanf("") : (sum > 0.f ? 1.0f / sum : 0.f);
       *reinterpret_cast<u32x2*>(out + ((size_t)(n0 + t) * Hq + hk * G + c - t * G) * DH + d) =
           u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
     } else {
-      const size_t slot = (((size_t)tile * Hkv + hk) * ranges + rng) * max_cols + c;
-      *reinterpret_cast<f32x4*>(ws_o + slot * DH + d) = o;
-      if (d == 0) {
-        ws_ml[2 * slot] = nan ? __builtin_nanf("") : top;
-        ws_ml[2 * slot + 1] = sum;
+      const size_t slot = (part0 + rng) * max_cols + c;
+      put_through(ws_o + slot * DH + d, o[0], o[1]);
+      put_through(ws_o + slot * DH + d + 2, o[2], o[3]);
+      if (d == 0) put_through(ws_ml + 2 * slot, nan ? __builtin_nanf("") : top, sum);
+    }
+  }
+  if (alone) return;
+
+  // Every wavefront waits until its stores have got to where all compute units read them (vmcnt(0)), then the barrier, then
+  // one thread takes a ticket, atomically for the whole GPU: whoever takes the last one knows that all parts are there, and
+  // reads them past its own die's caches.  It puts the counter back to zero for the next launch.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __syncthreads();  // (also: nobody reads ml any more)
+  int* last_flag = reinterpret_cast<int*>(ml);
+  if (threadIdx.x == 0) {
+    int* ticket = tickets + (size_t)tile * Hkv + hk;
+    const bool is_last = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == mine - 1;
+    if (is_last) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *last_flag = is_last;
+  }
+  __syncthreads();
+  if (!*last_flag) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  f32x2* parts = reinterpret_cast<f32x2*>(smem);  // [mine][cols]: the parts' maxima and sums
+  for (int i = threadIdx.x; i < mine * cols; i += W * 64) {
+    const int r = i / cols, c = i - r * cols;
+    parts[i] = get_through(ws_ml + 2 * ((part0 + r) * max_cols + c));
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < cols * (DH / 2); i += W * 64) {
+    const int c = i / (DH / 2), d = 2 * (i - c * (DH / 2));
+    const float* po = ws_o + (part0 * max_cols + c) * DH + d;
+    float top = -INFINITY, sum = 0.f;
+    bool nan = false;
+    for (int r = 0; r < mine; ++r) {
+      const float mr = parts[r * cols + c][0];
+      nan |= mr != mr;
+      top = fmaxf(top, mr);
+    }
+    const float use = top == -INFINITY ? 0.f : top;
+    f32x2 o = {0.f, 0.f};
+    for (int r0 = 0; r0 < mine; r0 += 8) {  // eight parts' numbers on their way at once, added up in the ranges' order
+      f32x2 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = get_through(po + (size_t)min(r0 + k, mine - 1) * max_cols * DH);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const f32x2 part = parts[min(r0 + k, mine - 1) * cols + c];
+        const float f = r0 + k < mine ? __builtin_amdgcn_exp2f(part[0] - use) : 0.f;
+        sum = fmaf(part[1], f, sum);
+        o[0] = fmaf(v[k][0], f, o[0]);
+        o[1] = fmaf(v[k][1], f, o[1]);
       }
     }
-  }
-}
-
-// The ranges' results of every (tile, kv head, column), added up in the ranges' order: a wavefront each.
-__global__ __launch_bounds__(256) void attention_quantized_merge_kernel(
-    const float* __restrict__ ws_ml, const float* __restrict__ ws_o, bf16_t* __restrict__ out,
-    const int* __restrict__ positions, const int* __restrict__ tiles, int num_tiles, int ranges, int range, int ret_mode,
-    int ret_param, int Hq, int Hkv, int DH, int max_cols) {
-  const int lane = threadIdx.x & 63;
-  const int item = blockIdx.x * 4 + wave_index();
-  if (item >= num_tiles * Hkv * max_cols) return;
-  const int c = item % max_cols, hk = item / max_cols % Hkv, tile = item / (max_cols * Hkv);
-  const int n0 = tiles[2 * tile], nt = tiles[2 * tile + 1];
-  const int G = Hq / Hkv;
-  if (c >= nt * G) return;
-  const int p_first = positions[n0];
-  const int first = first_key(ret_mode, ret_param, p_first);
-  const int ns = (p_first + nt - 1) / range - first / range + 1;
-  const size_t slot0 = ((size_t)tile * Hkv + hk) * ranges * max_cols + c;
-  float top = -INFINITY;
-  bool nan = false;
-  for (int r = lane; r < ns; r += 64) {
-    const float mr = ws_ml[2 * (slot0 + (size_t)r * max_cols)];
-    nan |= mr != mr;
-    top = fmaxf(top, mr);
-  }
-  top = wave_max(top);
-  nan = __any(nan);
-  const float use = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  for (int r = lane; r < ns; r += 64)
-    sum = fmaf(ws_ml[2 * (slot0 + (size_t)r * max_cols) + 1],
-               __builtin_amdgcn_exp2f(ws_ml[2 * (slot0 + (size_t)r * max_cols)] - use), sum);
-  sum = wave_sum(sum);
-  const float inv = nan ? __builtin_nanf("") : (sum > 0.f ? 1.0f / sum : 0.f);
-  const int t = c / G;
-  bf16_t* dst = out + ((size_t)(n0 + t) * Hq + hk * G + c - t * G) * DH;
-  for (int d = 4 * lane; d < DH; d += 256) {
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int r = 0; r < ns; ++r) {
-      const float f = __builtin_amdgcn_exp2f(ws_ml[2 * (slot0 + (size_t)r * max_cols)] - use);
-      const f32x4 v = *reinterpret_cast<const f32x4*>(ws_o + (slot0 + (size_t)r * max_cols) * DH + d);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = fmaf(v[e], f, o[e]);
-    }
-    *reinterpret_cast<u32x2*>(dst + d) = u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
+    const float inv = nan ? __builtin_nanf("") : (sum > 0.f ? 1.0f / sum : 0.f);
+    const int t = over(c, group);
+    *reinterpret_cast<uint32_t*>(out + ((size_t)(n0 + t) * Hq + hk * G + c - t * G) * DH + d) = pack_bf16(o[0] * inv, o[1] * inv);
   }
 }
 
 // tiles: [num_tiles][2] = (first row, tokens), tokens * Hq / Hkv <= max_cols <= 64 (32 for heads of 256); every tile's
 // tokens are consecutive positions of one segment.  ranges: the most ranges of `range` positions (a multiple of 32) that a
-// tile reads.  ws_ml: [num_tiles][Hkv][ranges][max_cols][2], ws_o: the same with [dh]; null with one range.
+// tile reads.  ws_ml: [num_tiles][Hkv][ranges][max_cols][2], ws_o: the same with [dh], tickets: [num_tiles][Hkv], zero before
+// and after; null with one range.  tiles null: tile i is the single token i.  waves: of a block (4 or 8, up to 16 columns; 0:
+// as many as suit).
 JLE_API int jle_attention_quantized(const void* q, const void* codes, const void* scales, void* out, float* ws_ml,
-                                    float* ws_o, const int* positions, const int* token_segment, const int* block_table,
+                                    float* ws_o, int* tickets, const int* positions, const int* token_segment, const int* block_table,
                                     int table_width, int num_pages, const int* tiles, int num_tiles, int max_cols,
                                     int ranges, int range, int ret_mode, int ret_param, float scale, int Hq, int Hkv,
-                                    int dh, int ps, hipStream_t s) {
+                                    int dh, int ps, int waves, hipStream_t s) {
   if (num_tiles <= 0) return 0;
   if (!quantized_head_ok(dh) || Hkv <= 0 || Hq % Hkv || ps < 16 || ps % 16 || max_cols < Hq / Hkv) return JLE_BAD_ARG;
-  if (max_cols > (dh == 256 ? 32 : 64) || ranges < 1 || range < 32 || range % 32 || num_pages <= 0) return JLE_BAD_ARG;
-  if (ranges > 1 && (ws_ml == nullptr || ws_o == nullptr)) return JLE_BAD_ARG;
+  if (table_width < 1 || max_cols > (dh == 256 ? 32 : 64) || ranges < 1 || range < 32 || range % 32 || num_pages <= 0) return JLE_BAD_ARG;
+  if (ranges > 1 && (ws_ml == nullptr || ws_o == nullptr || tickets == nullptr)) return JLE_BAD_ARG;
+  if (waves != 0 && waves != 4 && waves != 8) return JLE_BAD_ARG;
   if ((ret_mode == 1 || ret_mode == 2) && ret_param <= 0) return JLE_BAD_ARG;
+  if (((uintptr_t)ws_ml | (uintptr_t)ws_o) & 7) return JLE_BAD_ARG;
   if (!(scale > 0.f) || (((uintptr_t)q | (uintptr_t)codes | (uintptr_t)scales | (uintptr_t)out) & 15)) return JLE_BAD_ARG;
-  const long long blocks = (long long)num_tiles * Hkv * ranges;
-  if (blocks > (1ll << 30)) return JLE_BAD_ARG;
+  if (num_tiles > 65535 || ranges > kMostRanges) return JLE_BAD_ARG;
   const float sl = scale * kLog2e;
+  const Rule rule = {ret_mode, divisor(ret_mode == 0 ? 1 : ret_param)};
 #define LAUNCH(DH, CT, W)                                                                                                   \
   do {                                                                                                                      \
     const size_t lds = (size_t)(W) * max_cols * ((DH) + 4 + 2) * sizeof(float);                                             \
     const int rc = allow_lds(attention_quantized_kernel<DH, CT, W>, lds);                                                   \
     if (rc) return rc;                                                                                                      \
-    hipLaunchKernelGGL((attention_quantized_kernel<DH, CT, W>), dim3((unsigned)blocks), dim3((W) * 64), lds, s,             \
-                       (const bf16_t*)q, (const uint8_t*)codes, (const uint8_t*)scales, (bf16_t*)out, ws_ml, ws_o,          \
-                       positions, token_segment, block_table, table_width, num_pages, tiles, ranges, range, ret_mode,       \
-                       ret_param, sl, Hq, Hkv, ps, max_cols);                                                               \
+    hipLaunchKernelGGL((attention_quantized_kernel<DH, CT, W>), dim3(Hkv, num_tiles, ranges), dim3((W) * 64), lds, s,             \
+                       (const bf16_t*)q, (const uint8_t*)codes, (const uint8_t*)scales, (bf16_t*)out, ws_ml, ws_o, tickets, \
+                       positions, token_segment, block_table, table_width, num_pages, tiles, ranges, divisor(range), rule, sl, Hq, Hkv,    \
+                       divisor(Hq / Hkv), divisor(ps / 16), max_cols);                                                      \
   } while (0)
 #define PICK(DH)                               \
   do {                                         \
-    if (max_cols <= 16) LAUNCH(DH, 1, 8);      \
-    else if (max_cols <= 32) LAUNCH(DH, 2, 8); \
+    if (max_cols <= 16 && waves == 4) LAUNCH(DH, 1, 4); \
+    else if (max_cols <= 16) LAUNCH(DH, 1, 8); \
+    else if (max_cols <= 32) LAUNCH(DH, 2, (DH) <= 96 ? 8 : 4); \
     else LAUNCH(DH, 4, 4);                     \
   } while (0)
   switch (dh) {
@@ -380,12 +434,5 @@ JLE_API int jle_attention_quantized(const void* q, const void* codes, const void
 #undef PICK
 #undef LAUNCH
   JLE_LAUNCH_CHECK();
-  if (ranges > 1) {
-    const long long items = (long long)num_tiles * Hkv * max_cols;
-    if (items > (1ll << 30)) return JLE_BAD_ARG;
-    hipLaunchKernelGGL(attention_quantized_merge_kernel, dim3((unsigned)((items + 3) / 4)), dim3(256), 0, s, ws_ml, ws_o,
-                       (bf16_t*)out, positions, tiles, num_tiles, ranges, range, ret_mode, ret_param, Hq, Hkv, dh, max_cols);
-    JLE_LAUNCH_CHECK();
-  }
   return 0;
 }

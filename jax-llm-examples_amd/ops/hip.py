@@ -132,10 +132,11 @@ _SIGNATURES = {
     "jle_attention_prefill_kept": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _vp, _i, _i, _i, _f, _i, _i, _i, _i, _vp],
     "jle_paged_attention_kept": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _f, _i, _i, _i, _i, _i, _i, _i, _i, _vp,
                                  _vp, _vp],
-    "jle_quantized_prepare": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _vp, _vp, _i, _i, _f, _f, _i, _i, _i, _i, _i, _i, _vp],
+    "jle_quantized_prepare": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _vp, _vp, _i, _i, _f, _f, _i, _i, _i, _i, _i, _i, _vp,
+                              _i, _vp],
     "jle_quantized_read": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
-    "jle_attention_quantized": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i,
-                                _i, _vp],
+    "jle_attention_quantized": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _i,
+                                _i, _i, _i, _vp],
     "jle_paged_attention_biased": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _i, _i, _i, _i, _i, _i, _i, _i, _vp,
                                    _vp, _vp, _i, _vp, _f, _vp],
 }
@@ -267,6 +268,7 @@ class HipOps:
         # counters of the kernels in which the last wavefront (or block) to finish does the closing work: zero
         # between launches (whoever closes puts its counter back), so they are cleared here once
         self._tickets = torch.zeros(self.TICKETS, dtype=torch.int32, device=self.device)
+        self._quantized_sizes: set = set()  # (query heads, kv heads, head size, page size) that the kernels over codes take
         self._slice_tickets = torch.zeros(self.SLICE_TICKETS, dtype=torch.int32, device=self.device)
         self._compute_units = torch.cuda.get_device_properties(self.device).multi_processor_count
         torch.backends.cuda.matmul.allow_tf32 = False
@@ -311,6 +313,8 @@ class HipOps:
 
     @staticmethod
     def _chk(t: torch.Tensor, dtype=None, shape=None, what: str = "tensor") -> torch.Tensor:
+        if t.is_cuda and t.is_contiguous() and (dtype is None or t.dtype == dtype) and (shape is None or t.shape == shape):
+            return t
         if not t.is_cuda:
             raise KernelError(f"{what} must be on the GPU")
         if not t.is_contiguous():
@@ -2202,9 +2206,17 @@ class HipOps:
         ``prep`` says, k and v written into their pages (if this run ``writes`` its cache), attention over the
         pages.  A step of single tokens in bfloat16 is one launch (``attention_decode_fused_kernel``)."""
         if isinstance(kv_cache, QuantizedPages):
+            tickets, retention = None, tuple(retention)
+            if qkv.shape[0]:  # (the preparation clears the counters of the attention behind it)
+                self._chk_quantized(kv_cache, num_heads, num_kv_heads, head_dim)
+                self._chk(block_table, torch.int32, None, "block table")
+                plan = self._quantized_plan_of(meta, token_segment, positions, retention, num_heads, kv_cache, block_table)
+                if plan["tickets"]:
+                    tickets = torch.empty(plan["tickets"], dtype=torch.int32, device=qkv.device)
             q = self._qk_prepare_quantized(qkv, num_heads, num_kv_heads, head_dim, positions, prep, kv_cache, slot_mapping,
-                                           writes)
-            return self.paged_attention(q, kv_cache, block_table, positions, token_segment, retention, scale, meta)
+                                           writes, tickets)
+            return self._attention_quantized(q, kv_cache, block_table, positions, token_segment, retention, scale, meta,
+                                             tickets)
         n = qkv.shape[0]
         hq, hk, dh = num_heads, num_kv_heads, head_dim
         ps = kv_cache.shape[3]
@@ -2555,26 +2567,30 @@ class HipOps:
 
     # ------------------------------------------------------------------ keys and values in 8 bits
     def _chk_quantized(self, kv, num_heads: int, num_kv_heads: int, head_dim: int) -> None:
-        self._chk(kv.codes, torch.uint8, None, "codes")
-        if kv.device != self._tickets.device:
-            raise KernelError(f"pages on {kv.device}, the kernels run on {self._tickets.device}")
-        if kv.shape[2] != num_kv_heads or kv.shape[4] != head_dim:
-            raise KernelError(f"pages of {kv.shape[2]} kv heads of {kv.shape[4]}, asked for {num_kv_heads} of {head_dim}")
-        try:
-            _quantized.check_sizes(num_heads, num_kv_heads, head_dim, kv.shape[3])
-        except ValueError as e:
-            raise KernelError(str(e)) from None
+        self._here(kv.codes, "pages")
+        _, _, hk, ps, dh = kv.shape
+        if hk != num_kv_heads or dh != head_dim:
+            raise KernelError(f"pages of {hk} kv heads of {dh}, asked for {num_kv_heads} of {head_dim}")
+        if (num_heads, hk, dh, ps) not in self._quantized_sizes:
+            try:
+                _quantized.check_sizes(num_heads, hk, dh, ps)
+            except ValueError as e:
+                raise KernelError(str(e)) from None
+            self._quantized_sizes.add((num_heads, hk, dh, ps))
+
+    def _here(self, t, what: str) -> None:
+        if t.device != self._tickets.device:
+            raise KernelError(f"{what} must be on the GPU that the kernels run on, {self._tickets.device}, not on {t.device}")
+        if t.data_ptr() % 16:
+            raise KernelError(f"{what} must be aligned to 16 bytes")
 
     def _chk16(self, t, dtype, shape, what: str):
         self._chk(t, dtype, shape, what)
-        if t.device != self._tickets.device:
-            raise KernelError(f"{what} on {t.device}, the kernels run on {self._tickets.device}")
-        if t.data_ptr() % 16:
-            raise KernelError(f"{what} must be aligned to 16 bytes")
+        self._here(t, what)
         return t
 
     def _qk_prepare_quantized(self, qkv, num_heads, num_kv_heads, head_dim, positions, prep, kv, slot_mapping,
-                              writes: bool = True):
+                              writes: bool = True, clear=None):
         n = qkv.shape[0]
         hq, hk, dh = num_heads, num_kv_heads, head_dim
         self._chk_quantized(kv, hq, hk, dh)
@@ -2605,7 +2621,7 @@ class HipOps:
                    _p(kv.scales) if writes else None, _p(positions), _p(slot_mapping) if writes else None, _p(inv_freq),
                    -1.0 if prep.norm_eps is None else float(prep.norm_eps), int(bool(prep.norm_first)),
                    _p(prep.norm_weight_q), _p(prep.norm_weight_k), pairing, rd, float(fs), float(sc), n, hq, hk, dh,
-                   kv.shape[3], kv.shape[0])
+                   kv.shape[3], kv.shape[0], _p(clear), 0 if clear is None else clear.numel())
         return q
 
     def read_pages(self, kv: QuantizedPages, page_ids):
@@ -2627,14 +2643,41 @@ class HipOps:
         return out
 
     QUANTIZED_COLUMNS = 64  # a segment whose tokens times query heads a kv head are no more takes the kernel over codes
-    QUANTIZED_STEPS = (256, 4096)  # keys of a block's range: at least, at most
-    QUANTIZED_KEY_US, QUANTIZED_MERGE_US, QUANTIZED_RESULT_US = 0.02, 4.0, 0.05
+    QUANTIZED_RANGES = 128  # of a (tile, kv head), at most
+    # measured on MI355X at head size 128: a block of eight wavefronts works through a key in 4.8 ns, however many blocks there
+    # are (98 to 32,768 keys of 8 kv heads), all of them together through 6.4 TB/s; a block begins and ends in 3.5 us, and
+    # ranges that hand each other results cost 3 us and 0.1 us a range
+    QUANTIZED_KEY_US, QUANTIZED_BYTES_PER_US, QUANTIZED_BLOCK_US = 0.0048, 6.4e6, 3.5
+    QUANTIZED_MERGE_US, QUANTIZED_RESULT_US = 3.0, 0.1
+
+    def _quantized_split(self, spans, num_kv_heads: int, head_dim: int):
+        """How many keys a range of a (tile, kv head) has: ``spans(keys)`` says how many ranges of so many keys each tile has
+        and how many keys that is in all.  Returns ``(the most ranges of a tile, keys a range, wavefronts a block)``."""
+        best, keys = None, 256
+        while True:
+            each, total = spans(keys)
+            most = max(each)
+            if most <= self.QUANTIZED_RANGES:
+                blocks = num_kv_heads * sum(each)
+                rounds = -(-blocks // self._compute_units)
+                cost = max(rounds * (self.QUANTIZED_BLOCK_US + min(keys, total) * self.QUANTIZED_KEY_US * head_dim / 128),
+                           self.QUANTIZED_BLOCK_US
+                           + num_kv_heads * total * 2 * _quantized.bytes_per_row(head_dim) / self.QUANTIZED_BYTES_PER_US)
+                if most > 1:
+                    cost += self.QUANTIZED_MERGE_US + self.QUANTIZED_RESULT_US * most
+                if best is None or cost < best[0]:
+                    # four rounds of blocks and more: smaller blocks, three of which share a compute unit (128 requests of
+                    # 2,048 keys 92 -> 85 us, 64 of 6,100 135 -> 138)
+                    best = (cost, most, keys, 4 if rounds >= 4 else 8)
+                if most == 1:
+                    return best[1:]
+            keys += 256 if keys < 2048 else keys
 
     def _quantized_plan(self, seg_lens, seg_starts, retention, num_kv_heads: int, group: int, head_dim: int, page_size: int,
                         decode_bucket, block_table):
         """What a step's attention over pages in 8 bits is made of.  ``few``: for segments of few tokens, by the columns that
-        a wavefront takes (16, 32, 64), ``(tiles, number, columns, ranges, keys a range)``; ``long``: for the others, the
-        tiles of the attention kernel over pages in bfloat16, the pages it needs read back and the block table over those."""
+        a wavefront takes (16, 32, 64), their tiles, the most columns, the ranges; ``long``: for the others, the tiles of the
+        attention kernel over pages in bfloat16, the pages it needs read back and the block table over those."""
         from ..parts.base import first_needed_position
 
         device = block_table.device
@@ -2647,30 +2690,23 @@ class HipOps:
         for i, n in enumerate(seg_lens):
             if n <= tokens:
                 cols = 16 if n * group <= 16 else 32 if n * group <= 32 else 64
-                start = None if seg_starts is None else seg_starts[i]
-                few.setdefault(cols, []).append((o, n, start))
+                few.setdefault(cols, []).append((o, n, None if seg_starts is None else seg_starts[i]))
             o += n
         plan = {"few": [], "long": None}
         for cols, items in sorted(few.items()):
-            if decode_bucket is not None:
-                of = lambda cand: [self._most_ranges(retention, decode_bucket, cand)] * len(items)
+            if decode_bucket is not None:  # (the same for all steps of so many requests below this bound)
+                held = decode_bucket if retention[0] == "all" else min(decode_bucket, int(retention[1]))
+                spans = lambda keys: ([self._most_ranges(retention, decode_bucket, keys)] * len(items), held * len(items))
             else:
-                spans = [(first_needed_position(retention, s), s + n - 1) for _, n, s in items]
-                of = lambda cand: [last // cand - first // cand + 1 for first, last in spans]
-            best = None
-            low, high = self.QUANTIZED_STEPS
-            cand = low
-            while cand <= high:
-                r = of(cand)
-                blocks = num_kv_heads * sum(r)
-                cost = (-(-blocks // self._compute_units) * cand * self.QUANTIZED_KEY_US
-                        + (self.QUANTIZED_MERGE_US + self.QUANTIZED_RESULT_US * max(r) if max(r) > 1 else 0.0))
-                if best is None or cost <= best[0]:
-                    best = (cost, cand, max(r))
-                cand += low
-            flat = [x for at, n, _ in items for x in (at, n)]
-            plan["few"].append((to_device(torch.from_numpy(np.array(flat, np.int32)), device), len(items),
-                                max(n for _, n, _ in items) * group, best[2], best[1]))
+                ends = [(first_needed_position(retention, s), s + n - 1) for _, n, s in items]
+                spans = lambda keys: ([last // keys - first // keys + 1 for first, last in ends],
+                                      sum(last - first + 1 for first, last in ends))
+            ranges, keys, waves = self._quantized_split(spans, num_kv_heads, head_dim)
+            tiles = None  # (tile i is token i)
+            if len(items) != len(seg_lens) or any(n != 1 for n in seg_lens):
+                tiles = to_device(torch.from_numpy(np.array([x for at, n, _ in items for x in (at, n)], np.int32)), device)
+            plan["few"].append((tiles, len(items), max(n for _, n, _ in items) * group, ranges, keys, waves, {}))
+        plan["tickets"] = sum(num * num_kv_heads for _, num, _, ranges, _, _, _ in plan["few"] if ranges > 1)
         if any(n > tokens for n in seg_lens):
             ps, width = page_size, block_table.shape[1]
             where = []
@@ -2689,40 +2725,61 @@ class HipOps:
             plan["long"] = (tiles, where, table)
         return plan
 
-    def _attention_quantized(self, q, kv, block_table, positions, token_segment, retention, scale: float, meta):
-        n, hq, dh = q.shape
-        p, _, hk, ps, _ = kv.shape
-        self._chk_quantized(kv, hq, hk, dh)
-        self._chk16(q, torch.bfloat16, (n, hq, dh), "q (over a cache in 8 bits)")
-        self._chk(block_table, torch.int32, None, "block table")
-        self._chk(positions, torch.int32, (n,), "positions")
-        self._chk(token_segment, torch.int32, (n,), "token segments")
-        if retention[0] == "window_keep":
-            raise KernelError("attention over a cache in 8 bits reads keys under the rules all, chunk and window")
-        if not scale > 0:
-            raise KernelError("attention over a cache in 8 bits takes a positive softmax scale")
-        mode = _ret_mode(retention)
-        param = int(retention[1]) if len(retention) > 1 else 0
-        out = torch.empty(n, hq * dh, dtype=q.dtype, device=q.device)
-        if n == 0:
-            return out
-        key = ("quantized_plan", tuple(retention), hk, hq // hk, dh, ps)
+    def _quantized_plan_of(self, meta, token_segment, positions, retention, hq: int, kv, block_table):
+        _, _, hk, ps, dh = kv.shape
+        key = ("quantized_plan", retention, hk, hq // hk, dh, ps)
         plan = meta.meta.get(key) if meta is not None else None
         if plan is None:
+            if retention[0] == "window_keep":
+                raise KernelError("attention over a cache in 8 bits reads keys under the rules all, chunk and window")
+            _ret_mode(retention)
             bucket = meta.decode_bucket if meta is not None else None
             seg_lens, seg_starts = (meta.seg_lens, None) if bucket is not None else self._segments(meta, token_segment, positions)
             plan = self._quantized_plan(seg_lens, seg_starts, retention, hk, hq // hk, dh, ps, bucket, block_table)
             if meta is not None:
                 meta.meta[key] = plan
-        for tiles, num, cols, ranges, span in plan["few"]:
-            ws_ml = ws_o = None
+        return plan
+
+    def _attention_quantized(self, q, kv, block_table, positions, token_segment, retention, scale: float, meta, tickets=None):
+        """``tickets``: as many zeros as the plan says, for this call alone."""
+        n, hq, dh = q.shape
+        p, _, hk, ps, _ = kv.shape
+        self._chk_quantized(kv, hq, hk, dh)
+        self._chk16(q, torch.bfloat16, None, "q (over a cache in 8 bits)")
+        self._chk(block_table, torch.int32, None, "block table")
+        self._chk(positions, torch.int32, (n,), "positions")
+        self._chk(token_segment, torch.int32, (n,), "token segments")
+        if not scale > 0:
+            raise KernelError("attention over a cache in 8 bits takes a positive softmax scale")
+        out = torch.empty(n, hq * dh, dtype=torch.bfloat16, device=q.device)
+        if n == 0:
+            return out
+        retention = tuple(retention)
+        plan = self._quantized_plan_of(meta, token_segment, positions, retention, hq, kv, block_table)
+        mode = _RET_MODES[retention[0]]
+        param = int(retention[1]) if mode else 0
+        used = 0
+        for tiles, num, cols, ranges, span, waves, kept in plan["few"]:
+            ws_ml = ws_o = mine = None
             if ranges > 1:
                 slots = num * hk * ranges * cols
-                ws_ml = torch.empty(slots * 2, dtype=torch.float32, device=q.device)
-                ws_o = torch.empty(slots * dh, dtype=torch.float32, device=q.device)
-            self._call("jle_attention_quantized", _p(q), _p(kv.codes), _p(kv.scales), _p(out), _p(ws_ml), _p(ws_o),
+                ws_o = torch.empty(slots * (dh + 2), dtype=torch.float32, device=q.device)
+                ws_ml = ws_o.data_ptr() + slots * dh * 4
+                if tickets is not None:
+                    mine = tickets.data_ptr() + 4 * used
+                    used += num * hk
+                elif torch.cuda.is_current_stream_capturing():
+                    # (a recorded call's own: two recordings may run at once)
+                    tickets_now = torch.zeros(num * hk, dtype=torch.int32, device=q.device)
+                    mine = tickets_now.data_ptr()
+                else:  # a stream's calls with this plan follow each other, and each leaves zeros
+                    stream = self._stream()
+                    if stream not in kept:
+                        kept[stream] = torch.zeros(num * hk, dtype=torch.int32, device=q.device)
+                    mine = kept[stream].data_ptr()
+            self._call("jle_attention_quantized", _p(q), _p(kv.codes), _p(kv.scales), _p(out), ws_ml, _p(ws_o), mine,
                        _p(positions), _p(token_segment), _p(block_table), block_table.shape[1], p, _p(tiles), num, cols,
-                       ranges, span, mode, param, float(scale), hq, hk, dh, ps)
+                       ranges, span, mode, param, float(scale), hq, hk, dh, ps, waves)
         if plan["long"] is not None:
             tiles, where, table = plan["long"]
             pages = self._read_pages(kv, block_table, where)

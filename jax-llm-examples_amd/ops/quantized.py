@@ -46,7 +46,8 @@ def check_sizes(num_heads: int, num_kv_heads: int, head_dim: int, page_size: int
 @dataclasses.dataclass(frozen=True)
 class QuantizedPages:
     """``codes``: uint8 ``[pages, kv_heads, 2, page_size, head_dim]`` (the last two in :func:`places`' order, sixteen keys
-    after sixteen), ``scales``: uint8 ``[pages, kv_heads, 2, page_size]``; index 0 holds keys, 1 values."""
+    after sixteen), ``scales``: uint8 ``[pages, kv_heads, 2, page_size]``; index 0 holds keys, 1 values.  ``shape`` is that of
+    pages in the run dtype, ``[pages, 2, kv_heads, page_size, head_dim]``."""
 
     codes: torch.Tensor
     scales: torch.Tensor
@@ -58,6 +59,9 @@ class QuantizedPages:
                              f"[pages, kv_heads, 2, page_size], not {c.dtype} {tuple(c.shape)} and {s.dtype} {tuple(s.shape)}")
         if c.device != s.device or not c.is_contiguous() or not s.is_contiguous():
             raise ValueError("the codes and scales of pages in 8 bits are contiguous and on one device")
+        p, hk, two, ps, dh = c.shape
+        object.__setattr__(self, "shape", torch.Size((p, two, hk, ps, dh)))
+        object.__setattr__(self, "device", c.device)
 
     @classmethod
     def empty(cls, num_pages: int, kv_heads: int, page_size: int, head_dim: int, device, poison: bool = False):
@@ -66,16 +70,6 @@ class QuantizedPages:
         fill = NAN_CODE if poison else 0  # (as a scale byte: 1)
         new = lambda *shape: torch.full((num_pages, kv_heads, 2, page_size, *shape), fill, dtype=torch.uint8, device=device)
         return cls(new(head_dim), new())
-
-    @property
-    def shape(self) -> torch.Size:
-        """As the pages of the run dtype have it: ``[pages, 2, kv_heads, page_size, head_dim]``."""
-        p, hk, two, ps, dh = self.codes.shape
-        return torch.Size((p, two, hk, ps, dh))
-
-    @property
-    def device(self):
-        return self.codes.device
 
     def poison_(self, pages: torch.Tensor) -> None:
         """What the given pages hold reads as NaN from now on."""

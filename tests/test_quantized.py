@@ -375,7 +375,7 @@ def test_refused_on_the_gpu(ops):
         ops.qk_prepare_kv_write(rows, 4, 2, 64, pos, QKPreparation(rotation=Rotation(torch.ones(32, device=DEV), magnitude=2.0)), c.kv, pos)
     with pytest.raises(KernelError, match="bfloat16"):
         ops.qk_prepare_kv_write(rows.float(), 4, 2, 64, pos, QKPreparation(), c.kv, pos)
-    with pytest.raises(KernelError, match="must be on the GPU"):
+    with pytest.raises(KernelError, match="must be on the GPU that"):
         ops.read_pages(QuantizedPages(c.kv.codes.cpu(), c.kv.scales.cpu()), pos)
     with pytest.raises(KernelError, match="page ids"):
         ops.read_pages(c.kv, pos.long())
