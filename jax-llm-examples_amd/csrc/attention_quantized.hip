@@ -20,18 +20,6 @@
 
 using namespace jle;
 
-// x / d for 0 <= x < 2^31 by a product: with floor(2^32 / d) (2^32 - 1 for one) the estimate is the quotient or one less.
-// (A division of two numbers that are only known when the kernel runs is tens of instructions, and a short launch waits for
-// every instruction that it meets for the first time.)
-struct Divisor {
-  uint32_t d, magic;
-};
-static Divisor divisor(int d) { return {(uint32_t)d, d == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (uint32_t)d)}; }
-__device__ __forceinline__ int over(int x, Divisor by) {
-  const uint32_t q = __umulhi((uint32_t)x, by.magic);
-  return (int)(q + ((uint32_t)x - q * by.d >= by.d));
-}
-
 // The first key that a query at `pos` reads: rules all (0), chunk (1), window (2).
 struct Rule {
   int mode;

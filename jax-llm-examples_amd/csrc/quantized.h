@@ -47,6 +47,18 @@ __device__ __forceinline__ uint32_t pack_codes(float a, float b, float c, float 
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 
+// x / d for 0 <= x < 2^31 by a product: with floor(2^32 / d) (2^32 - 1 for one) the estimate is the quotient or one less.
+// (A division of two numbers that are only known when the kernel runs is tens of instructions, and a short launch waits for
+// every instruction that it meets for the first time.)
+struct Divisor {
+  uint32_t d, magic;
+};
+inline Divisor divisor(int d) { return {(uint32_t)d, d == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (uint32_t)d)}; }
+__device__ __forceinline__ int over(int x, Divisor by) {
+  const uint32_t q = __umulhi((uint32_t)x, by.magic);
+  return (int)(q + ((uint32_t)x - q * by.d >= by.d));
+}
+
 __host__ inline bool quantized_head_ok(int dh) { return dh == 32 || dh == 64 || dh == 96 || dh == 128 || dh == 256; }
 
 }  // namespace jle

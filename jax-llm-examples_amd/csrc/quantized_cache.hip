@@ -54,10 +54,12 @@ struct PrepareArgs {
   const float* inv_freq;  // null: no rotation
   const float *norm_wq, *norm_wk;
   float norm_eps;  // < 0: no norm
+  double per_element;  // 1 / dh
   float floor_scale, attn_scale;
-  int norm_first, pairing, rotary_dim;  // pairing 0: (x[2j], x[2j + 1]), 1: (x[j], x[j + rotary_dim / 2])
+  int norm_first, table_pairs, pairing, rotary_dim;  // pairing 0: (x[2j], x[2j + 1]), 1: (x[j], x[j + rotary_dim / 2])
   int N, Hq, Hkv, dh, ps;
   long long num_slots;
+  Divisor key_chunks, value_quads;  // of a head: eight codes; (piece of 64 elements, element % 16)
   int* clear;  // counters of the attention behind this launch, which it starts from zero
   int num_clear;
 };
@@ -72,107 +74,143 @@ __device__ __forceinline__ F over_head(F s) {
   return s;
 }
 
-// A head's numbers, eight a lane (l: the lane's place in the head), normed and turned.  F: what is computed in.
-template <typename F, int LPH>
-__device__ __forceinline__ void prepare_head(F (&x)[8], const PrepareArgs& a, const float* w, int l, bool live, const double2* turns) {
-  auto norm = [&]() {
+// 1 / sqrt(x): the hardware's estimate; in 64 bits two steps of Newton's method behind it
+__device__ __forceinline__ float inverse_root(float x) { return __builtin_amdgcn_rsqf(x); }
+__device__ __forceinline__ double inverse_root(double x) {
+  double r = __builtin_amdgcn_rsq(x);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) r = fma(0.5 * r, fma(-x * r, r, 1.0), r);
+  return r;
+}
+
+// A head's numbers, eight a lane (l: the lane's place in the head), normed and turned.  F: what is computed in.  A rotation
+// changes no length, so the norm's sum is that of the numbers as they come, whether the norm lies in front of the rotation or
+// behind it; only its weights have a place.  turns: (cosine, sine) by pair; adjacent pairs beyond the rotated part: (1, 0).
+template <typename F, int LPH, typename T2>
+__device__ __forceinline__ void prepare_head(F (&x)[8], const PrepareArgs& a, const float* w, int l, bool live, const T2* turns) {
+  F mul = 1;
+  if (a.norm_eps >= 0.f) {
     F ss = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ss = fma(x[i], x[i], ss);
-    ss = over_head<F, LPH>(ss);
-    const F mul = F(1) / sqrt(ss / (F)a.dh + (F)a.norm_eps);
+    mul = inverse_root(fma(over_head<F, LPH>(ss), (F)a.per_element, (F)a.norm_eps));
+  }
+  auto weigh = [&]() {
+    const uint32_t at = live ? 8 * l : 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= w != nullptr && live ? mul * (F)w[8 * l + i] : mul;
+    for (int i = 0; i < 8; ++i) x[i] *= (F)w[at + i];
   };
-  if (a.norm_eps >= 0.f && a.norm_first) norm();
+  if (w != nullptr && a.norm_first) weigh();
   if (a.inv_freq != nullptr) {
     if (a.pairing == 0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (8 * l + 2 * i < a.rotary_dim) {
-          const double2 t = turns[4 * l + i];  // (cosine, sine)
-          const F p = x[2 * i], q = x[2 * i + 1], c = (F)t.x, s = (F)t.y;
-          x[2 * i] = fma(p, c, -(q * s));
-          x[2 * i + 1] = fma(q, c, p * s);
-        }
+        const T2 t = turns[live ? 4 * l + i : 0];
+        const F p = x[2 * i], q = x[2 * i + 1], c = (F)t.x, s = (F)t.y;
+        x[2 * i] = fma(p, c, -(q * s));
+        x[2 * i + 1] = fma(q, c, p * s);
       }
     } else {  // (half of the rotated part is a multiple of 8: a lane's partners are all in one other lane)
       const int half = a.rotary_dim >> 1, lane = threadIdx.x & 63;
       const bool turned = 8 * l < a.rotary_dim, leading = 8 * l < half;
       const int other = turned ? (leading ? lane + half / 8 : lane - half / 8) : lane;
+      const T2* mine = turns + (leading ? 8 * l : turned ? 8 * l - half : 0);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const F y = __shfl(x[i], other, 64);
-        if (turned) {
-          const double2 t = turns[leading ? 8 * l + i : 8 * l + i - half];
-          x[i] = fma(x[i], (F)t.x, (leading ? -y : y) * (F)t.y);
-        }
+        const T2 t = mine[i];
+        x[i] = turned ? fma(x[i], (F)t.x, (leading ? -y : y) * (F)t.y) : x[i];
       }
     }
   }
-  if (a.norm_eps >= 0.f && !a.norm_first) norm();
+  if (w != nullptr && !a.norm_first) weigh();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] *= mul;
 }
 
-// A block takes TB consecutive tokens; LPH lanes a head (a power of two, at least dh / 8), eight neighbouring elements a lane,
-// 64 / LPH heads of a kind (queries, keys, values) a wavefront at a time: a *unit*.  The block's sines and cosines are formed
-// once.  With one token a block (few tokens) the units are shared out among gridDim.y blocks and the codes go straight into
-// their pages; with several the codes are gathered in shared memory and written in pieces of 16 bytes: keys a token's sixteen
-// elements, values the four keys of four elements where the block's tokens fill an aligned four of a page (other values byte
-// by byte).
-template <int LPH, int TB>
-__global__ __launch_bounds__(256) void quantized_prepare_kernel(PrepareArgs a) {
-  constexpr int HPW = 64 / LPH;
+// LPH lanes a head (a power of two, at least dh / 8), eight neighbouring elements a lane, 64 / LPH heads of a kind (queries,
+// keys, values) a wavefront at a time: a *unit*.  A block takes TB consecutive tokens and forms their sines and cosines once.
+// With one token a block (few tokens) the units are shared out among gridDim.y blocks of four wavefronts and the codes go
+// straight into their pages; with several TW wavefronts share a token, the codes are gathered in shared memory and written
+// in larger pieces: keys eight codes each, the tokens' side by side, values the four keys of four elements in 16 bytes where
+// the block's tokens fill an aligned four of a page (other values byte by byte).
+template <int LPH, int TB, int TW>
+__global__ __launch_bounds__(TB > 1 ? TB * 64 * TW : 256, 4) void quantized_prepare_kernel(PrepareArgs a) {
+  constexpr int HPW = 64 / LPH, THREADS = TB > 1 ? TB * 64 * TW : 256;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int lane = threadIdx.x & 63, wave = wave_index();
   const int l = lane & (LPH - 1), sub = lane / LPH;
-  const int n0 = blockIdx.x * TB, half = a.rotary_dim >> 1;
-  const int H = a.Hq + 2 * a.Hkv, dh = a.dh, row_codes = a.Hkv * dh;
-  double2* turns = reinterpret_cast<double2*>(smem);         // [TB][half]
-  uint8_t* held = smem + (size_t)TB * half * sizeof(double2);  // [2][TB][Hkv][dh], several tokens only
+  const int n0 = blockIdx.x * TB;
+  const int pairs = a.table_pairs, half = a.rotary_dim >> 1;  // of a token's table; of them turned
+  const int dh = a.dh, row_codes = a.Hkv * dh;
+  double2* turns = reinterpret_cast<double2*>(smem);  // [TB][pairs]: for keys, and in float32 for queries
+  float2* turns32 = reinterpret_cast<float2*>(turns + TB * pairs);
+  uint8_t* held = reinterpret_cast<uint8_t*>(turns32 + TB * pairs);  // [2][TB][Hkv][dh], several tokens only
   __shared__ int slot_of[TB], leads[TB];
+  __shared__ float temper[TB];
+  __shared__ size_t code_at[TB];  // of head 0's keys of the slot's sixteen
   if (a.num_clear > 0 && blockIdx.y == 0)
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < a.num_clear; i += gridDim.x * 256) a.clear[i] = 0;
+    for (int i = blockIdx.x * THREADS + threadIdx.x; i < a.num_clear; i += gridDim.x * THREADS) a.clear[i] = 0;
 
-  const int uq = (a.Hq + HPW - 1) / HPW, uk = a.codes != nullptr ? (a.Hkv + HPW - 1) / HPW : 0;
-  const int units = uq + 2 * uk, all = TB * units;
-  const int stride = 4 * gridDim.y;
-  const bool in_head = 8 * l < dh;
+  const int tk = TB > 1 ? wave / TW : 0, n = n0 + tk;
+  const int uq = (a.Hq + HPW - 1) / HPW, uk = a.codes != nullptr ? (a.Hkv + HPW - 1) / HPW : 0, units = uq + 2 * uk;
+  const int step = TB > 1 ? TW : 4 * gridDim.y;
+  const bool in_head = 8 * l < dh, token = n < a.N;
   constexpr int AHEAD = TB > 1 ? 4 : 1;  // units' rows asked for at once
-  for (int i = threadIdx.x; i < TB * half; i += 256) {
-    const int tk = i / half;
-    if (n0 + tk < a.N) {
-      double sn, cs;
-      turn_of(a.positions[n0 + tk], a.inv_freq[i - tk * half], sn, cs);
+  u32x4 raw[AHEAD], next[AHEAD];
+  const uint32_t in_unit = sub * dh + 8 * l;  // a lane's first element among a unit's
+  const bf16_t* row = a.qkv + (size_t)(token ? n : 0) * (a.Hq + 2 * a.Hkv) * dh;
+  // a unit's kind, its first head and, of those, how many there are
+  auto unit = [&](int u, int& kind, int& h0) {
+    kind = u < uq ? 0 : u < uq + uk ? 1 : 2;
+    h0 = (kind == 0 ? u : u - uq - (kind - 1) * uk) * HPW;
+    return min((kind == 0 ? a.Hq : a.Hkv) - h0, HPW);
+  };
+  auto ask = [&](u32x4 (&raw)[AHEAD], int first) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      int kind, h0;
+      const int u = first + k * step, heads = unit(u, kind, h0);
+      raw[k] = u32x4{0u, 0u, 0u, 0u};
+      if (u < units && token && sub < heads && in_head)
+        raw[k] = *reinterpret_cast<const u32x4*>(row + ((kind == 0 ? 0 : a.Hq + (kind - 1) * a.Hkv) + h0) * dh + in_unit);
+    }
+  };
+  const int first0 = TB > 1 ? wave % TW : wave + 4 * blockIdx.y;
+  ask(raw, first0);  // (on their way while the angles are formed)
+  for (int i = threadIdx.x; i < TB * pairs; i += THREADS) {
+    const int t = TB > 1 ? i / pairs : 0, j = i - t * pairs;
+    if (n0 + t < a.N) {
+      double sn = 0.0, cs = 1.0;
+      if (j < half) turn_of(a.positions[n0 + t], a.inv_freq[j], sn, cs);
       turns[i] = double2{cs, sn};
+      turns32[i] = float2{(float)cs, (float)sn};
     }
   }
-  if (TB > 1 && threadIdx.x < TB) {
-    const int n = n0 + threadIdx.x;
-    long long s = n < a.N && a.codes != nullptr ? a.slots[n] : -1;
-    slot_of[threadIdx.x] = s >= 0 && s < a.num_slots ? (int)s : -1;
+  if (threadIdx.x < TB) {
+    const int m = n0 + threadIdx.x;
+    const long long s = m < a.N && a.codes != nullptr ? a.slots[m] : -1;
+    const int slot = s >= 0 && s < a.num_slots ? (int)s : -1;
+    const int page = slot < 0 ? 0 : slot / a.ps, off = slot < 0 ? 0 : slot - page * a.ps;
+    slot_of[threadIdx.x] = slot;
+    code_at[threadIdx.x] = ((size_t)page * a.Hkv * 2 * a.ps + (off & ~15)) * dh;
+    temper[threadIdx.x] = a.floor_scale > 0.f && m < a.N
+                              ? 1.0f + a.attn_scale * log1pf(floorf(((float)a.positions[m] + 1.0f) / a.floor_scale)) : 1.f;
   }
   __syncthreads();
 
-  for (int first = wave + 4 * blockIdx.y; first < all; first += AHEAD * stride) {
-    u32x4 raw[AHEAD];
+  const int slot = slot_of[tk];
+  const size_t plane_codes = (size_t)a.ps * dh, at = code_at[tk];
+  // (of head 0's keys: the slot's scale byte)
+  const size_t scale_at = at / (uint32_t)dh + (uint32_t)(slot & 15);
+  for (int first = first0; token && first < units; first += AHEAD * step) {
+    ask(next, first + AHEAD * step);
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
-      const int at = first + k * stride, tk = at / units, u = at - tk * units;
-      const int kind = u < uq ? 0 : u < uq + uk ? 1 : 2;
-      const int h = (kind == 0 ? u : u - uq - (kind - 1) * uk) * HPW + sub;
-      const bool live = at < all && n0 + tk < a.N && h < (kind == 0 ? a.Hq : a.Hkv) && in_head;
-      raw[k] = u32x4{0u, 0u, 0u, 0u};
-      if (live)
-        raw[k] = *reinterpret_cast<const u32x4*>(a.qkv + ((size_t)(n0 + tk) * H + (kind == 0 ? 0 : a.Hq + (kind - 1) * a.Hkv) + h) * dh + 8 * l);
-    }
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      const int at = first + k * stride, tk = at / units, u = at - tk * units;
-      const int n = n0 + tk;
-      if (at >= all || n >= a.N) continue;  // (the same in all lanes)
-      const int kind = u < uq ? 0 : u < uq + uk ? 1 : 2;
-      const int h = (kind == 0 ? u : u - uq - (kind - 1) * uk) * HPW + sub;
-      const bool live = h < (kind == 0 ? a.Hq : a.Hkv) && in_head;
+      const int u = first + k * step;
+      if (u >= units) break;
+      int kind, h0;
+      const bool live = sub < unit(u, kind, h0) && in_head;
       float x[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -180,22 +218,19 @@ __global__ __launch_bounds__(256) void quantized_prepare_kernel(PrepareArgs a) {
         x[2 * i + 1] = __uint_as_float(raw[k][i] & 0xffff0000u);
       }
       if (kind == 0) {
-        prepare_head<float, LPH>(x, a, a.norm_wq, l, live, turns + tk * half);
-        if (a.floor_scale > 0.f) {
-          const float mul = 1.0f + a.attn_scale * log1pf(floorf(((float)a.positions[n] + 1.0f) / a.floor_scale));
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] *= mul;
-        }
+        prepare_head<float, LPH>(x, a, a.norm_wq, l, live, turns32 + tk * pairs);
+        const float mul = temper[tk];
         if (live)
-          *reinterpret_cast<u32x4*>(a.q_out + ((size_t)n * a.Hq + h) * dh + 8 * l) =
-              u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
+          *reinterpret_cast<u32x4*>(a.q_out + ((size_t)n * a.Hq + h0) * dh + in_unit) =
+              u32x4{pack_bf16(x[0] * mul, x[1] * mul), pack_bf16(x[2] * mul, x[3] * mul), pack_bf16(x[4] * mul, x[5] * mul),
+                    pack_bf16(x[6] * mul, x[7] * mul)};
         continue;
       }
       if (kind == 1) {
         double y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = x[i];
-        prepare_head<double, LPH>(y, a, a.norm_wk, l, live, turns + tk * half);
+        prepare_head<double, LPH>(y, a, a.norm_wk, l, live, turns + tk * pairs);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = (float)y[i];
       }
@@ -204,36 +239,28 @@ __global__ __launch_bounds__(256) void quantized_prepare_kernel(PrepareArgs a) {
       for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
 #pragma unroll
       for (int o = LPH >> 1; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-      if (!live) continue;
-      long long slot;
-      if (TB > 1) {
-        slot = slot_of[tk];
-      } else {
-        slot = a.slots[n];
-        if (slot >= a.num_slots) slot = -1;
-      }
-      if (slot < 0) continue;
-      const int byte = scale_byte(top);
+      if (!live || slot < 0) continue;
+      const int byte = scale_byte(top), plane = 2 * (h0 + sub) + kind - 1;
       const float f = code_factor(byte);
       u32x2 c = {kCodesNaN, kCodesNaN};
       if (byte < 255) c = u32x2{pack_codes(x[0] * f, x[1] * f, x[2] * f, x[3] * f), pack_codes(x[4] * f, x[5] * f, x[6] * f, x[7] * f)};
-      const int which = kind - 1, page = (int)(slot / a.ps), off = (int)(slot - (long long)page * a.ps);
-      const size_t plane = ((size_t)page * a.Hkv + h) * 2 + which;
-      if (l == 0) a.scales[plane * a.ps + off] = (uint8_t)(byte < 255 ? byte : 127);
+      if (l == 0) a.scales[scale_at + (size_t)plane * a.ps] = (uint8_t)(byte < 255 ? byte : 127);
       if (TB > 1) {
-        *reinterpret_cast<u32x2*>(held + (size_t)(which * TB + tk) * row_codes + h * dh + 8 * l) = c;
+        *reinterpret_cast<u32x2*>(held + ((kind - 1) * TB + tk) * row_codes + h0 * dh + in_unit) = c;
       } else {
-        uint8_t* block = a.codes + (plane * a.ps + (off & ~15)) * dh;
-        if (which == 0) {
-          *reinterpret_cast<u32x2*>(block + key_place(8 * l, off & 15, dh)) = c;
+        uint8_t* block = a.codes + at + plane * plane_codes;
+        if (kind == 1) {
+          *reinterpret_cast<u32x2*>(block + key_place(8 * l, slot & 15, dh)) = c;
         } else {
-          uint8_t* dst = block + value_place(8 * l, off & 15, dh);
+          uint8_t* dst = block + value_place(8 * l, slot & 15, dh);
           const int u2 = lane_codes(8 * l, dh);
 #pragma unroll
           for (int i = 0; i < 8; ++i) dst[i * u2] = (uint8_t)((i < 4 ? c[0] : c[1]) >> (8 * (i & 3)));
         }
       }
     }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) raw[k] = next[k];
   }
   if (TB == 1 || a.codes == nullptr) return;
 
@@ -252,98 +279,105 @@ __global__ __launch_bounds__(256) void quantized_prepare_kernel(PrepareArgs a) {
     leads[r] = lead;
   }
   __syncthreads();
-  auto block_of = [&](int slot, int h, int which) {
-    const int page = slot / a.ps, off = slot - page * a.ps;
-    return a.codes + ((((size_t)page * a.Hkv + h) * 2 + which) * a.ps + (off & ~15)) * dh;
-  };
-  const int chunks = dh / 8;
-  for (int i = threadIdx.x; i < TB * a.Hkv * chunks; i += 256) {  // keys: eight codes, tokens next to each other
-    const int tk = i % TB, c = i / TB % chunks, h = i / (TB * chunks);
-    const int slot = slot_of[tk];
-    if (slot >= 0)
-      *reinterpret_cast<u32x2*>(block_of(slot, h, 0) + key_place(8 * c, slot & 15, dh)) =
-          *reinterpret_cast<const u32x2*>(held + (size_t)tk * row_codes + h * dh + 8 * c);
+  {  // keys: eight codes, tokens next to each other
+    const int t = threadIdx.x % TB, mine = slot_of[t], chunks = dh / 8;
+    uint8_t* page = a.codes + code_at[t];
+    if (mine >= 0)
+      for (int i = threadIdx.x / TB; i < a.Hkv * chunks; i += THREADS / TB) {
+        const int h = over(i, a.key_chunks), c = i - h * chunks;
+        *reinterpret_cast<u32x2*>(page + 2 * h * plane_codes + key_place(8 * c, mine & 15, dh)) =
+            *reinterpret_cast<const u32x2*>(held + t * row_codes + h * dh + 8 * c);
+      }
   }
-  const int quads = (dh + 63) / 64 * 16;  // (piece, element % 16) pairs
-  for (int i = threadIdx.x; i < TB * a.Hkv * quads; i += 256) {
-    const int e = i % quads, h = i / quads % a.Hkv, tk = i / (quads * a.Hkv);
-    const int slot = slot_of[tk], lead = leads[tk];
-    if (slot < 0 || lead == 1) continue;
+  const int quads = (int)a.value_quads.d;  // (piece, element % 16) pairs of a head
+  for (int i = threadIdx.x; i < a.Hkv * quads; i += THREADS) {
+    const int h = over(i, a.value_quads), e = i - h * quads;
     const int d = e / 16 * 64 + (e & 15), u = lane_codes(d, dh);
-    const uint8_t* row = held + (size_t)(TB + tk) * row_codes + h * dh + d;
-    uint8_t* dst = block_of(slot, h, 1) + value_place(d, slot & 15, dh);
-    if (lead == 2) {
-      u32x4 v = {0u, 0u, 0u, 0u};
+#pragma unroll 2
+    for (int t = 0; t < TB; ++t) {
+      const int mine = slot_of[t], lead = leads[t];
+      if (mine < 0 || lead == 1) continue;
+      const uint8_t* row = held + (TB + t) * row_codes + h * dh + d;
+      uint8_t* dst = a.codes + code_at[t] + (2 * h + 1) * plane_codes + value_place(d, mine & 15, dh);
+      if (lead == 2) {
+        u32x4 v = {0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (4 * j < u)
-          v[j] = row[16 * j] | row[row_codes + 16 * j] << 8 | row[2 * row_codes + 16 * j] << 16 |
-                 (uint32_t)row[3 * row_codes + 16 * j] << 24;
-      if (u == 16) *reinterpret_cast<u32x4*>(dst) = v;
-      else *reinterpret_cast<u32x2*>(dst) = u32x2{v[0], v[1]};
-    } else {
-      for (int j = 0; 4 * j < u; ++j) dst[4 * j] = row[16 * j];
+        for (int j = 0; j < 4; ++j)
+          if (4 * j < u)
+            v[j] = row[16 * j] | row[row_codes + 16 * j] << 8 | row[2 * row_codes + 16 * j] << 16 |
+                   (uint32_t)row[3 * row_codes + 16 * j] << 24;
+        if (u == 16) *reinterpret_cast<u32x4*>(dst) = v;
+        else *reinterpret_cast<u32x2*>(dst) = u32x2{v[0], v[1]};
+      } else {
+        for (int j = 0; 4 * j < u; ++j) dst[4 * j] = row[16 * j];
+      }
     }
   }
 }
 
 // Pages in bfloat16, in the layout of the attention kernels (keys [page_size][dh], values [dh][page_size]; every number is
-// exact).  A wavefront takes sixteen keys of one (page, kv head), keys or values.  Page i is page_ids[where[i]] (where null:
-// page_ids[i]); an id that is no page's gives NaN.
+// exact).  Page i is page_ids[where[i]] (where null: page_ids[i]); an id that is no page's gives NaN.  An item is 16 bytes of
+// the result: eight elements of a key, or eight keys of an element of the values; blockIdx: (page, part of its items, keys or
+// values), and a page's items follow each other in the result's order, so that every store of a wavefront is one kilobyte
+// (values of pages of sixteen: with pages of 16 and more tokens a row of theirs, 32 bytes and more).
+constexpr int kReadItems = 4;  // of a thread
+__device__ __forceinline__ uint32_t two_bf16(uint32_t w, float scale, bool hi) {
+  return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true)
+                                         : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
+}
 __global__ __launch_bounds__(256) void quantized_read_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                              const int* __restrict__ page_ids,
                                                              const int* __restrict__ where, bf16_t* __restrict__ out,
-                                                             long long items, int num_pages, int Hkv, int ps, int dh) {
-  const long long item = (long long)blockIdx.x * 4 + wave_index();
-  if (item >= items) return;
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int blocks = ps / 16;
-  const int kb = (int)(item % blocks);
-  const long long i2 = item / blocks;
-  const int hk = (int)(i2 % Hkv);
-  const long long i3 = i2 / Hkv;
-  const int which = (int)(i3 & 1);
-  const long long i = i3 >> 1;
-  const int page = page_ids[where != nullptr ? where[i] : (int)i];
+                                                             int num_pages, int Hkv, int ps, int dh, Divisor plane_items,
+                                                             Divisor row_keys, Divisor row_values) {
+  const int i = blockIdx.x, which = blockIdx.z;
+  const int page = page_ids[where != nullptr ? where[i] : i];
   const bool ok = page >= 0 && page < num_pages;
-  const size_t plane = ((size_t)(ok ? page : 0) * Hkv + hk) * 2 + which;
-  const uint8_t* src = codes + (plane * ps + 16 * kb) * dh;
-  const uint8_t* sc = scales + plane * ps + 16 * kb;
-  bf16_t* dst = out + (((size_t)i * 2 + which) * Hkv + hk) * ps * dh;
-  float f[4];  // keys: the lane's one; values: its four
-  if (which == 0) {
-    f[0] = f[1] = f[2] = f[3] = ok ? scale_of(sc[r]) : 1.f;
-  } else {
-    const uint32_t b = *reinterpret_cast<const uint32_t*>(sc + 4 * g);
+  const int items = Hkv * (int)plane_items.d;
+  const size_t plane_codes = (size_t)ps * dh;
+  const uint8_t* cp = codes + ((size_t)(ok ? page : 0) * Hkv * 2 + which) * plane_codes;  // head h: + 2 h planes
+  const uint8_t* sp = scales + ((size_t)(ok ? page : 0) * Hkv * 2 + which) * ps;
+  bf16_t* dst = out + ((size_t)i * 2 + which) * Hkv * plane_codes;
+  const int first = blockIdx.y * (256 * kReadItems) + threadIdx.x;
+  u32x2 c[kReadItems], f[kReadItems];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = ok ? scale_of((b >> (8 * j)) & 255u) : 1.f;
+  for (int k = 0; k < kReadItems; ++k) {  // everything is asked for before the first item is worked on
+    const int at = min(first + 256 * k, items - 1);
+    const int h = over(at, plane_items), r = at - h * (int)plane_items.d;
+    const uint8_t* plane = cp + 2 * h * plane_codes;
+    const uint8_t* row_scales = sp + 2 * h * ps;
+    if (which == 0) {
+      const int key = over(r, row_keys), d = 8 * (r - key * (int)row_keys.d);
+      c[k] = *reinterpret_cast<const u32x2*>(plane + (key & ~15) * dh + key_place(d, key & 15, dh));
+      f[k][0] = row_scales[key];
+    } else {
+      const int d = over(r, row_values), key = 8 * (r - d * (int)row_values.d);
+      const uint8_t* p = plane + (key & ~15) * dh + value_place(d, key & 15, dh);
+      c[k][0] = *reinterpret_cast<const uint32_t*>(p);
+      c[k][1] = *reinterpret_cast<const uint32_t*>(p + 16 * lane_codes(d, dh));
+      f[k] = *reinterpret_cast<const u32x2*>(row_scales + key);
+    }
   }
-  for (int d0 = 0; d0 < dh; d0 += 64) {
-    const int u = lane_codes(d0, dh);
-    uint32_t w[4] = {kCodesNaN, kCodesNaN, kCodesNaN, kCodesNaN};
-    if (ok) {
-      const uint8_t* p = src + d0 * 16 + lane * u;
-      if (u == 16) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(p);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = v[j];
-      } else {
-        const u32x2 v = *reinterpret_cast<const u32x2*>(p);
-        w[0] = v[0];
-        w[1] = v[1];
+  for (int k = 0; k < kReadItems; ++k) {
+    const int at = first + 256 * k;
+    if (at >= items) break;
+    u32x4 v;
+    if (which == 0) {
+      const float s = scale_of(f[k][0]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = two_bf16(c[k][j >> 1], s, j & 1);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const auto x = (j & 1) ? __builtin_amdgcn_cvt_pk_f32_fp8((int)c[k][j >> 1], true)
+                               : __builtin_amdgcn_cvt_pk_f32_fp8((int)c[k][j >> 1], false);
+        const uint32_t b = f[k][j >> 1] >> (16 * (j & 1));
+        v[j] = pack_bf16(x[0] * scale_of(b & 255u), x[1] * scale_of((b >> 8) & 255u));
       }
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (4 * j >= u) break;
-      const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[j], false);
-      const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[j], true);
-      const u32x2 b = {pack_bf16(lo[0] * f[0], lo[1] * f[1]), pack_bf16(hi[0] * f[2], hi[1] * f[3])};
-      if (which == 0)
-        *reinterpret_cast<u32x2*>(dst + (size_t)(16 * kb + r) * dh + d0 + u * g + 4 * j) = b;
-      else
-        *reinterpret_cast<u32x2*>(dst + (size_t)(d0 + 16 * j + r) * ps + 16 * kb + 4 * g) = b;
-    }
+    if (!ok) v = u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+    *reinterpret_cast<u32x4*>(dst + 8 * (size_t)at) = v;
   }
 }
 
@@ -365,21 +399,29 @@ JLE_API int jle_quantized_prepare(const void* qkv, void* q_out, void* codes, voi
   if (rotary_dim < 0 || rotary_dim % 2 || rotary_dim > dh || (pairing != 0 && pairing != 1)) return JLE_BAD_ARG;
   if (pairing == 1 && rotary_dim % 16) return JLE_BAD_ARG;
   const int lph = dh == 32 ? 4 : dh == 64 ? 8 : dh == 256 ? 32 : 16;
+  const int pairs = inv_freq == nullptr ? 0 : pairing == 0 ? dh / 2 : rotary_dim / 2;
   const PrepareArgs a = {(const bf16_t*)qkv, (bf16_t*)q_out, (uint8_t*)codes, (uint8_t*)scales, positions, slot_mapping,
-                         inv_freq, norm_wq, norm_wk, norm_eps, floor_scale, attn_scale, norm_first, pairing, rotary_dim,
-                         N, Hq, Hkv, dh, ps, (long long)num_pages * ps, clear, num_clear};
+                         inv_freq, norm_wq, norm_wk, norm_eps, 1.0 / dh, floor_scale, attn_scale, norm_first, pairs, pairing, rotary_dim,
+                         N, Hq, Hkv, dh, ps, (long long)num_pages * ps, divisor(dh / 8), divisor((dh + 63) / 64 * 16),
+                         clear, num_clear};
   const int hpw = 64 / lph;
   const int units = (Hq + hpw - 1) / hpw + (codes != nullptr ? 2 * ((Hkv + hpw - 1) / hpw) : 0);
   // Several tokens a block from kManyTokens on, where their codes fit a quarter of the shared memory.
-  const size_t turns = (size_t)rotary_dim / 2 * sizeof(double2);
+  const size_t turns = (size_t)pairs * (sizeof(double2) + sizeof(float2));
   const size_t lds = kTokens * (turns + 2 * (size_t)Hkv * dh);
   const bool many = N >= kManyTokens && lds <= 40 * 1024;
-#define LAUNCH(LPH)                                                                                                     \
-  do {                                                                                                                  \
-    if (many)                                                                                                           \
-      hipLaunchKernelGGL((quantized_prepare_kernel<LPH, kTokens>), dim3((N + kTokens - 1) / kTokens), dim3(256), lds, s, a); \
-    else                                                                                                                \
-      hipLaunchKernelGGL((quantized_prepare_kernel<LPH, 1>), dim3(N, (units + 3) / 4), dim3(256), turns, s, a);          \
+  // two wavefronts a token while the blocks of eight are no more than two a compute unit (2,048 tokens of 40 + 16 heads 17.8 ->
+  // 15.6 us, 8,191 of 32 + 16 49 -> 60)
+  const bool wide = N <= 2 * 256 * kTokens;
+#define LAUNCH(LPH)                                                                                                        \
+  do {                                                                                                                     \
+    const dim3 blocks((N + kTokens - 1) / kTokens);                                                                        \
+    if (many && wide)                                                                                                      \
+      hipLaunchKernelGGL((quantized_prepare_kernel<LPH, kTokens, 2>), blocks, dim3(kTokens * 128), lds, s, a);             \
+    else if (many)                                                                                                         \
+      hipLaunchKernelGGL((quantized_prepare_kernel<LPH, kTokens, 1>), blocks, dim3(kTokens * 64), lds, s, a);              \
+    else                                                                                                                   \
+      hipLaunchKernelGGL((quantized_prepare_kernel<LPH, 1, 1>), dim3(N, (units + 3) / 4), dim3(256), turns, s, a);         \
   } while (0)
   switch (lph) {
     case 4: LAUNCH(4); break;
@@ -397,10 +439,12 @@ JLE_API int jle_quantized_read(const void* codes, const void* scales, const int*
   if (n <= 0) return 0;
   if (!jle_quantized_supported(dh, Hkv, Hkv, ps) || num_pages <= 0) return JLE_BAD_ARG;
   if (((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)out) & 15) return JLE_BAD_ARG;
-  const long long items = (long long)n * 2 * Hkv * (ps / 16);
-  if (items > (1ll << 32)) return JLE_BAD_ARG;
-  hipLaunchKernelGGL(quantized_read_kernel, dim3((unsigned)((items + 3) / 4)), dim3(256), 0, s, (const uint8_t*)codes,
-                     (const uint8_t*)scales, page_ids, where, (bf16_t*)out, items, num_pages, Hkv, ps, dh);
+  const long long items = (long long)Hkv * ps * (dh / 8);
+  const long long parts = (items + 256 * kReadItems - 1) / (256 * kReadItems);
+  if (parts > 65535) return JLE_BAD_ARG;
+  hipLaunchKernelGGL(quantized_read_kernel, dim3(n, (unsigned)parts, 2), dim3(256), 0, s, (const uint8_t*)codes,
+                     (const uint8_t*)scales, page_ids, where, (bf16_t*)out, num_pages, Hkv, ps, dh, divisor(ps * (dh / 8)),
+                     divisor(dh / 8), divisor(ps / 8));
   JLE_LAUNCH_CHECK();
   return 0;
 }
