@@ -395,7 +395,7 @@ JLE_API int jle_attention_quantized(const void* q, const void* codes, const void
 #define LAUNCH(DH, CT, W)                                                                                                   \
   do {                                                                                                                      \
     const size_t lds = (size_t)(W) * max_cols * ((DH) + 4 + 2) * sizeof(float);                                             \
-    const int rc = allow_lds(attention_quantized_kernel<DH, CT, W>, lds);                                                   \
+    const int rc = lds > 64 * 1024 ? allow_lds(attention_quantized_kernel<DH, CT, W>, lds) : 0;                             \
     if (rc) return rc;                                                                                                      \
     hipLaunchKernelGGL((attention_quantized_kernel<DH, CT, W>), dim3(Hkv, num_tiles, ranges), dim3((W) * 64), lds, s,             \
                        (const bf16_t*)q, (const uint8_t*)codes, (const uint8_t*)scales, (bf16_t*)out, ws_ml, ws_o, tickets, \

@@ -2762,22 +2762,25 @@ class HipOps:
         for tiles, num, cols, ranges, span, waves, kept in plan["few"]:
             ws_ml = ws_o = mine = None
             if ranges > 1:
+                # Counters (zero before and after every launch) and the ranges' results.  A recorded call has its own: two
+                # recordings may run at once.  Otherwise a stream's calls with this plan, which follow each other, share them.
                 slots = num * hk * ranges * cols
-                ws_o = torch.empty(slots * (dh + 2), dtype=torch.float32, device=q.device)
-                ws_ml = ws_o.data_ptr() + slots * dh * 4
+                stream = None if torch.cuda.is_current_stream_capturing() else self._stream()
+                held = kept.get(stream)
+                if held is None:
+                    held = (torch.empty(slots * (dh + 2), dtype=torch.float32, device=q.device),
+                            torch.zeros(num * hk, dtype=torch.int32, device=q.device)
+                            if stream is not None or tickets is None else None)
+                    if stream is not None:
+                        kept[stream] = held
+                ws_o = held[0].data_ptr()
+                ws_ml = ws_o + slots * dh * 4
                 if tickets is not None:
                     mine = tickets.data_ptr() + 4 * used
                     used += num * hk
-                elif torch.cuda.is_current_stream_capturing():
-                    # (a recorded call's own: two recordings may run at once)
-                    tickets_now = torch.zeros(num * hk, dtype=torch.int32, device=q.device)
-                    mine = tickets_now.data_ptr()
-                else:  # a stream's calls with this plan follow each other, and each leaves zeros
-                    stream = self._stream()
-                    if stream not in kept:
-                        kept[stream] = torch.zeros(num * hk, dtype=torch.int32, device=q.device)
-                    mine = kept[stream].data_ptr()
-            self._call("jle_attention_quantized", _p(q), _p(kv.codes), _p(kv.scales), _p(out), ws_ml, _p(ws_o), mine,
+                else:
+                    mine = held[1].data_ptr()
+            self._call("jle_attention_quantized", _p(q), _p(kv.codes), _p(kv.scales), _p(out), ws_ml, ws_o, mine,
                        _p(positions), _p(token_segment), _p(block_table), block_table.shape[1], p, _p(tiles), num, cols,
                        ranges, span, mode, param, float(scale), hq, hk, dh, ps, waves)
         if plan["long"] is not None:
