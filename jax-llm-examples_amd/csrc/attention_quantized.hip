@@ -371,7 +371,7 @@ __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
   }
 }
 
-// tiles: [num_tiles][2] = (first row, tokens), tokens * Hq / Hkv <= max_cols <= 64 (32 for heads of 256); every tile's
+// tiles: [num_tiles][2] = (first row, tokens), tokens * Hq / Hkv <= max_cols <= 32; every tile's
 // tokens are consecutive positions of one segment.  ranges: the most ranges of `range` positions (a multiple of 32) that a
 // tile reads.  ws_ml: [num_tiles][Hkv][ranges][max_cols][2], ws_o: the same with [dh], tickets: [num_tiles][Hkv], zero before
 // and after; null with one range.  tiles null: tile i is the single token i.  waves: of a block (4 or 8, up to 16 columns; 0:
@@ -383,7 +383,7 @@ JLE_API int jle_attention_quantized(const void* q, const void* codes, const void
                                     int dh, int ps, int waves, hipStream_t s) {
   if (num_tiles <= 0) return 0;
   if (!quantized_head_ok(dh) || Hkv <= 0 || Hq % Hkv || ps < 16 || ps % 16 || max_cols < Hq / Hkv) return JLE_BAD_ARG;
-  if (table_width < 1 || max_cols > (dh == 256 ? 32 : 64) || ranges < 1 || range < 32 || range % 32 || num_pages <= 0) return JLE_BAD_ARG;
+  if (table_width < 1 || max_cols > 32 || ranges < 1 || range < 32 || range % 32 || num_pages <= 0) return JLE_BAD_ARG;
   if (ranges > 1 && (ws_ml == nullptr || ws_o == nullptr || tickets == nullptr)) return JLE_BAD_ARG;
   if (waves != 0 && waves != 4 && waves != 8) return JLE_BAD_ARG;
   if ((ret_mode == 1 || ret_mode == 2) && ret_param <= 0) return JLE_BAD_ARG;
@@ -406,8 +406,7 @@ JLE_API int jle_attention_quantized(const void* q, const void* codes, const void
   do {                                         \
     if (max_cols <= 16 && waves == 4) LAUNCH(DH, 1, 4); \
     else if (max_cols <= 16) LAUNCH(DH, 1, 8); \
-    else if (max_cols <= 32) LAUNCH(DH, 2, (DH) <= 96 ? 8 : 4); \
-    else LAUNCH(DH, 4, 4);                     \
+    else LAUNCH(DH, 2, (DH) <= 96 ? 8 : 4);    \
   } while (0)
   switch (dh) {
     case 32: PICK(32); break;

@@ -2286,14 +2286,14 @@ class HipOps:
         return whole
 
     def attention_plan(self, seg_lens, seg_starts, retention, device, num_kv_heads=1, group_size=1, decode_bucket=None,
-                       tile=None, single_tiles=False, at_least=1):
+                       tile=None, single_tiles=False, only=None):
         """Work lists of the MFMA attention kernels for one step and one retention rule: the rows that are
         single decode tokens (and into how many keys their work is split; ``single_tiles``: these are tiles too), tiles of up
         to 32 consecutive tokens of longer segments and, with ``group_size`` > 1 query heads per kv head, the packing of the
         (tile, head) items of a kv head into blocks of wavefronts that share keys.  ``decode_bucket``: the step
         holds single tokens only, none beyond this context length: the split is then chosen from the number of
         tokens and this bound alone (not from where each request stands), so the same launch fits every such
-        step.  ``at_least``: segments of fewer tokens are left to another kernel."""
+        step.  ``only``: the others' segments are left to another kernel."""
         from ..parts.base import first_needed_position
 
         # (plain lists: of up to tens of segments they are laid out in half the time of arrays, 12 us a portion of 77 tokens)
@@ -2301,7 +2301,7 @@ class HipOps:
         tile = tile or self.PREFILL_TILE
         o = 0
         for i, n in enumerate(seg_lens):
-            if n < at_least:
+            if only is not None and i not in only:
                 pass
             elif n == 1 and not single_tiles:
                 dec.append(o)
@@ -2642,27 +2642,29 @@ class HipOps:
         self._call("jle_quantized_read", _p(kv.codes), _p(kv.scales), _p(page_ids), _p(where), _p(out), n, p, hk, dh, ps)
         return out
 
-    QUANTIZED_COLUMNS = 64  # a segment whose tokens times query heads a kv head are no more takes the kernel over codes
+    QUANTIZED_TOKENS = 512  # a segment of more tokens never takes the kernel over codes
     QUANTIZED_RANGES = 128  # of a (tile, kv head), at most
-    # measured on MI355X at head size 128: a block of eight wavefronts works through a key in 4.8 ns, however many blocks there
-    # are (98 to 32,768 keys of 8 kv heads), all of them together through 6.4 TB/s; a block begins and ends in 3.5 us, and
-    # ranges that hand each other results cost 3 us and 0.1 us a range
+    # measured on MI355X at head size 128, bfloat16 queries.  The kernel over codes: a block of eight wavefronts with up to 16
+    # columns works through a key in 4.8 ns (98 to 32,768 keys; with up to 32 columns in 8.9), all blocks together through
+    # 6.4 TB/s; a block begins and ends in 3.5 us, ranges that hand each other results cost 3 us and 0.1 us a range.  Pages read
+    # back and the attention over pages in bfloat16: 9 us, 26 ns a key of the longest segment (4,096 keys 113 us, 16,384 390),
+    # and 750 TFLOP/s, of which about 0.4 does not overlap
     QUANTIZED_KEY_US, QUANTIZED_BYTES_PER_US, QUANTIZED_BLOCK_US = 0.0048, 6.4e6, 3.5
     QUANTIZED_MERGE_US, QUANTIZED_RESULT_US = 3.0, 0.1
+    QUANTIZED_LONG_US, QUANTIZED_LONG_KEY_US, QUANTIZED_LONG_FLOPS_PER_US = 9.0, 0.026, 7.5e8
 
-    def _quantized_split(self, spans, num_kv_heads: int, head_dim: int):
-        """How many keys a range of a (tile, kv head) has: ``spans(keys)`` says how many ranges of so many keys each tile has
-        and how many keys that is in all.  Returns ``(the most ranges of a tile, keys a range, wavefronts a block)``."""
+    def _quantized_split(self, ranges_of, keys_of_all: int, keys_read: int, num_kv_heads: int, head_dim: int, wide: bool):
+        """How many keys a range of a (tile, kv head) has.  ``ranges_of(keys)``: how many ranges of so many keys the tiles have,
+        in all and at most; ``keys_of_all``: the tiles' keys, ``keys_read``: the same with those that tiles share counted once.
+        Returns ``(microseconds, the most ranges of a tile, keys a range, wavefronts a block)``."""
         best, keys = None, 256
+        key_us = self.QUANTIZED_KEY_US * head_dim / 128 * (1.85 if wide else 1.0)
+        read_us = num_kv_heads * keys_read * 2 * _quantized.bytes_per_row(head_dim) / self.QUANTIZED_BYTES_PER_US
         while True:
-            each, total = spans(keys)
-            most = max(each)
+            blocks, most = ranges_of(keys)
             if most <= self.QUANTIZED_RANGES:
-                blocks = num_kv_heads * sum(each)
-                rounds = -(-blocks // self._compute_units)
-                cost = max(rounds * (self.QUANTIZED_BLOCK_US + min(keys, total) * self.QUANTIZED_KEY_US * head_dim / 128),
-                           self.QUANTIZED_BLOCK_US
-                           + num_kv_heads * total * 2 * _quantized.bytes_per_row(head_dim) / self.QUANTIZED_BYTES_PER_US)
+                rounds = -(-num_kv_heads * blocks // self._compute_units)
+                cost = max(rounds * (self.QUANTIZED_BLOCK_US + min(keys, keys_of_all) * key_us), self.QUANTIZED_BLOCK_US + read_us)
                 if most > 1:
                     cost += self.QUANTIZED_MERGE_US + self.QUANTIZED_RESULT_US * most
                 if best is None or cost < best[0]:
@@ -2670,58 +2672,94 @@ class HipOps:
                     # 2,048 keys 92 -> 85 us, 64 of 6,100 135 -> 138)
                     best = (cost, most, keys, 4 if rounds >= 4 else 8)
                 if most == 1:
-                    return best[1:]
+                    return best
             keys += 256 if keys < 2048 else keys
 
     def _quantized_plan(self, seg_lens, seg_starts, retention, num_kv_heads: int, group: int, head_dim: int, page_size: int,
                         decode_bucket, block_table):
-        """What a step's attention over pages in 8 bits is made of.  ``few``: for segments of few tokens, by the columns that
-        a wavefront takes (16, 32, 64), their tiles, the most columns, the ranges; ``long``: for the others, the tiles of the
-        attention kernel over pages in bfloat16, the pages it needs read back and the block table over those."""
+        """What a step's attention over pages in 8 bits is made of.  ``few``: for single tokens and for segments of not so many
+        tokens that this kernel is the slower one, their tiles (as many tokens as 16 columns hold, or one), the columns, the
+        ranges; ``long``: for the others, the tiles of the attention kernel over pages in bfloat16, the pages that it needs
+        read back and the block table over those."""
         from ..parts.base import first_needed_position
 
         device = block_table.device
         if block_table.numel() >= 1 << 31:
             raise KernelError("a block table of 2^31 places and more")
-        most = min(self.QUANTIZED_COLUMNS, 32 if head_dim == 256 else 64)
-        tokens = max(1, most // group)
-        few = {}
-        o = 0
-        for i, n in enumerate(seg_lens):
-            if n <= tokens:
-                cols = 16 if n * group <= 16 else 32 if n * group <= 32 else 64
-                few.setdefault(cols, []).append((o, n, None if seg_starts is None else seg_starts[i]))
-            o += n
+        tokens = max(1, 16 // group)  # (tiles of 32 or 64 columns: slower from 16 tokens on 1,024 keys to 256 on 16,384)
+        wide = group > 16
+        offsets = np.concatenate([[0], np.cumsum(seg_lens)]).astype(np.int64)
+
+        def few_of(segments):
+            """Tiles ``(row, tokens, first key, last key)`` of the given segments, and their split."""
+            tiles = [(offsets[i] + t, min(tokens, seg_lens[i] - t), seg_starts[i] + t) for i in segments
+                     for t in range(0, seg_lens[i], tokens)]
+            first = np.array([first_needed_position(retention, s) for _, _, s in tiles])
+            last = np.array([s + n - 1 for _, n, s in tiles])
+
+            def ranges_of(keys):
+                each = last // keys - first // keys + 1
+                return int(each.sum()), int(each.max())
+
+            read = sum(seg_starts[i] + seg_lens[i] - first_needed_position(retention, seg_starts[i]) for i in segments)
+            return tiles, self._quantized_split(ranges_of, int((last - first + 1).sum()), read, num_kv_heads, head_dim, wide)
+
+        def long_us(segments):
+            if not segments:
+                return 0.0
+            keys = [seg_starts[i] + seg_lens[i] - first_needed_position(retention, seg_starts[i]) for i in segments]
+            serial = max(keys) * self.QUANTIZED_LONG_KEY_US
+            flops = (4.0 * num_kv_heads * group * head_dim * sum(k * seg_lens[i] for k, i in zip(keys, segments))
+                     / self.QUANTIZED_LONG_FLOPS_PER_US)
+            return self.QUANTIZED_LONG_US + max(serial, flops) + 0.4 * min(serial, flops)
+
         plan = {"few": [], "long": None}
-        for cols, items in sorted(few.items()):
-            if decode_bucket is not None:  # (the same for all steps of so many requests below this bound)
-                held = decode_bucket if retention[0] == "all" else min(decode_bucket, int(retention[1]))
-                spans = lambda keys: ([self._most_ranges(retention, decode_bucket, keys)] * len(items), held * len(items))
-            else:
-                ends = [(first_needed_position(retention, s), s + n - 1) for _, n, s in items]
-                spans = lambda keys: ([last // keys - first // keys + 1 for first, last in ends],
-                                      sum(last - first + 1 for first, last in ends))
-            ranges, keys, waves = self._quantized_split(spans, num_kv_heads, head_dim)
-            tiles = None  # (tile i is token i)
-            if len(items) != len(seg_lens) or any(n != 1 for n in seg_lens):
-                tiles = to_device(torch.from_numpy(np.array([x for at, n, _ in items for x in (at, n)], np.int32)), device)
-            plan["few"].append((tiles, len(items), max(n for _, n, _ in items) * group, ranges, keys, waves, {}))
+        long = []
+        if decode_bucket is not None:  # (single tokens; the same for all steps of so many requests below this bound)
+            n = len(seg_lens)
+            held = decode_bucket if retention[0] == "all" else min(decode_bucket, int(retention[1]))
+
+            def ranges_of(keys):
+                most = self._most_ranges(retention, decode_bucket, keys)
+                return most * n, most
+
+            split = self._quantized_split(ranges_of, held * n, held * n, num_kv_heads, head_dim, wide)
+            plan["few"].append((None, n, group, *split[1:], {}))
+        else:
+            # segments of up to so many tokens go through the kernel over codes: the bound with which the step is done first
+            short = [i for i, n in enumerate(seg_lens) if n <= tokens]
+            lengths = sorted({n for n in seg_lens if tokens < n <= self.QUANTIZED_TOKENS})
+            if len(lengths) > 6:
+                lengths = lengths[:: -(-len(lengths) // 6)] + lengths[-1:]
+            best = None
+            for bound in [tokens, *lengths]:
+                mine = short if bound == tokens else [i for i, n in enumerate(seg_lens) if n <= bound]
+                rest = [i for i, n in enumerate(seg_lens) if n > bound]
+                tiles, split = few_of(mine) if mine else ([], (0.0,))
+                cost = split[0] + long_us(rest)
+                if best is None or cost < best[0]:
+                    best = (cost, tiles, split, rest)
+            _, tiles, split, long = best
+            if tiles:
+                listed = None  # (tile i is token i)
+                if len(tiles) != len(seg_lens) or any(n != 1 for n in seg_lens):
+                    listed = to_device(torch.from_numpy(np.array([x for at, n, _ in tiles for x in (at, n)], np.int32)), device)
+                plan["few"].append((listed, len(tiles), max(n for _, n, _ in tiles) * group, *split[1:], {}))
         plan["tickets"] = sum(num * num_kv_heads for _, num, _, ranges, _, _, _ in plan["few"] if ranges > 1)
-        if any(n > tokens for n in seg_lens):
+        if long:
             ps, width = page_size, block_table.shape[1]
             where = []
-            for i, n in enumerate(seg_lens):
-                if n > tokens:
-                    first = first_needed_position(retention, seg_starts[i]) // ps
-                    last = min((seg_starts[i] + n - 1) // ps, width - 1)
-                    where.append(np.arange(i * width + first, i * width + last + 1, dtype=np.int32))
+            for i in long:
+                first = first_needed_position(retention, seg_starts[i]) // ps
+                last = min((seg_starts[i] + seg_lens[i] - 1) // ps, width - 1)
+                where.append(np.arange(i * width + first, i * width + last + 1, dtype=np.int32))
             where = np.concatenate(where)
             table = np.full(block_table.numel(), -1, np.int32)
             table[where] = np.arange(where.size, dtype=np.int32)
             sent = to_device(torch.from_numpy(np.concatenate([where, table])), device)
             where, table = sent[: where.size], sent[where.size:].view(block_table.shape)
             tiles = self.attention_plan(seg_lens, seg_starts, retention, device, num_kv_heads, group, single_tiles=True,
-                                        at_least=tokens + 1)
+                                        only=set(long))
             plan["long"] = (tiles, where, table)
         return plan
 
