@@ -245,7 +245,7 @@ def main() -> int:
     ap.add_argument("--serve", default="", help="requests through the scheduler, e.g. 64x512+128@64 (requests x prompt "
                     "+ output tokens @ decode batch), comma-separated: tokens a second end to end")
     ap.add_argument("--preset", default="llama4-scout")
-    ap.add_argument("--kv-dtype", default=None, help="hold keys and values in 8 bits (float8_e4m3) instead of the run dtype")
+    ap.add_argument("--kv-dtype", default=None, choices=["float8_e4m3"], help="hold keys and values in 8 bits (float8_e4m3) instead of the run dtype")
     ap.add_argument("--no-prefill", action="store_true")
     ap.add_argument("--design-points", default="1@2048,8@2048,64@2048", help="decode steps of --designs: batch@context")
     ap.add_argument("--designs", default="", help="instead of the default workload: prefill and decode of the Rovidra, "
@@ -254,6 +254,8 @@ def main() -> int:
     ap.add_argument("--design-names", default="", help="with --designs: only these of rovidra, tiradra, llama4-dense, "
                     "mazotar, llama4-moe, sudilorn, folivik, lifesun")
     args = ap.parse_args()
+    if args.designs and args.kv_dtype is not None:
+        raise SystemExit("--kv-dtype is for the default workload and its points, not for --designs")
     if args.designs:
         return bench_designs(args)
     if args.gpus != 1 or int(os.environ.get("WORLD_SIZE", "1")) != 1:

@@ -61,15 +61,16 @@ __device__ __forceinline__ f32x2 get_through(const float* p) {
   return __builtin_bit_cast(f32x2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
                                                      __HIP_MEMORY_SCOPE_AGENT));
 }
-constexpr int kMostRanges = 128;  // of a (tile, kv head): their maxima and sums fit where the wavefronts' results lay
+constexpr int kMostRanges = 64;  // of a (tile, kv head): their maxima and sums fit where the wavefronts' results lay
+
+static_assert(kMostRanges * sizeof(f32x2) <= 4 * (32 + 4) * sizeof(float), "a column's maxima and sums in its results' place");
 
 template <int DH, int CT, int W>
 __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
-    const bf16_t* __restrict__ q, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+    const bf16_t* q, const uint8_t* codes, const uint8_t* scales,
     bf16_t* __restrict__ out, float* __restrict__ ws_ml, float* __restrict__ ws_o, int* __restrict__ tickets,
-    const int* __restrict__ positions,
-    const int* __restrict__ token_segment, const int* __restrict__ block_table, int table_width, int num_pages,
-    const int* __restrict__ tiles, int ranges, Divisor range, Rule rule, float scale_log2, int Hq, int Hkv, Divisor group,
+    const int* __restrict__ positions, const int* __restrict__ token_segment, const int* __restrict__ block_table,
+    int table_width, int num_pages, const int* __restrict__ tiles, int ranges, Divisor range, Rule rule, float scale_log2, int Hq, int Hkv, Divisor group,
     Divisor page_tiles, int max_cols) {
   using Step = QuantizedStep<DH>;
   constexpr int P = Step::P, DT = DH / 16, KC = DH / 32, LD = DH + 4;
@@ -81,7 +82,8 @@ __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
   const int n0 = tiles != nullptr ? tiles[2 * tile] : tile, nt = tiles != nullptr ? tiles[2 * tile + 1] : 1;
   const int p_first = positions[n0], p_last = p_first + nt - 1;
   const int first = rule.first(p_first);
-  const int r_first = over(first, range), r_abs = r_first + rng, mine = over(p_last, range) - r_first + 1;
+  const int r_first = over(first, range), r_abs = r_first + rng;
+  const int all_ranges = over(p_last, range) - r_first + 1, mine = min(all_ranges, ranges);
   if (rng >= mine) return;  // (this tile has fewer ranges)
   const int k_lo = max(first, r_abs * (int)range.d), k_hi = min(p_last, r_abs * (int)range.d + (int)range.d - 1);
   const int full_lo = max(k_lo, rule.first(p_last)), full_hi = min(k_hi, p_first);
@@ -97,35 +99,33 @@ __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[ct][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  bool bad = false;
+  bool bad = all_ranges > ranges;  // (keys beyond what the launch was laid out for: the result is NaN)
   int lo[CT], hi[CT];
   bf16x8 qb[CT][KC];
 
   // The pages of a step are looked up, through the scalar path, two steps before their data is asked for: no load waits for
-  // the block table.  And every load is issued, whether its keys exist or not (then it reads page 0, and what it brings is
-  // masked or not used): the wait for one step's data then never includes the next one's.
+  // the block table.  And every load is issued, whether its keys exist or not (then it reads the range's nearest tile, and what
+  // it brings is masked or not used): the wait for one step's data then never includes the next one's.
   struct Pages {
     int id[2], off[2];  // per tile of sixteen keys: its page, the place of its first key there
   };
+  const int tile_lo = k_lo >> 4, tile_hi = k_hi >> 4;
+  bad |= over(tile_hi, page_tiles) >= table_width;
   auto look_up = [&](Pages& at, int step) {
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
-      const int key0 = 32 * step + 16 * tt;
-      const int idx = over(key0 >> 4, page_tiles);
-      const bool there = (key0 <= k_hi) & (key0 + 15 >= k_lo) & (idx < table_width);
-      const int id = table[there ? idx : 0];  // (without a branch; a table is at least one page wide)
-      at.id[tt] = there ? id : -1;
-      at.off[tt] = key0 - idx * ps;
+      const int kt = min(max(2 * step + tt, tile_lo), tile_hi), idx = over(kt, page_tiles);
+      at.id[tt] = table[min(idx, table_width - 1)];
+      at.off[tt] = 16 * (kt - idx * (int)page_tiles.d);
     }
   };
   const uint32_t page_rows = (uint32_t)Hkv * 2 * ps;
-  auto load = [&](Step& s, const Pages& at, int step) {
+  auto load = [&](Step& s, const Pages& at) {
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
-      const int key0 = 32 * step + 16 * tt, page = at.id[tt];
-      const bool ok = (page >= 0) & (page < num_pages);
-      bad |= !ok & (key0 <= k_hi) & (key0 + 15 >= k_lo);  // (a page is missing: the result is NaN)
-      const uint64_t row = (uint64_t)(uint32_t)(ok ? page : 0) * page_rows + (uint32_t)(hk * 2 * ps + (ok ? at.off[tt] : 0));
+      const bool ok = (uint32_t)at.id[tt] < (uint32_t)num_pages;
+      bad |= !ok;  // (a page is missing: the result is NaN)
+      const uint64_t row = (uint64_t)(uint32_t)(ok ? at.id[tt] : 0) * page_rows + (uint32_t)(hk * 2 * ps + at.off[tt]);
       const uint8_t* kp = codes + row * DH;
       const uint8_t* vp = kp + ps * DH;
       const uint8_t* sp = scales + row;
@@ -227,10 +227,11 @@ __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
 
   const int last = k_hi / 32;
   int step = k_lo / 32 + wave;
-  Step a, b;
-  Pages pa, pb;
-  look_up(pa, step);
-  look_up(pb, step + W);
+  constexpr int PF = 2;  // steps of a wavefront on their way or worked on (three: no faster, and a longer way in)
+  Step s[PF];
+  Pages at[PF];
+#pragma unroll
+  for (int k = 0; k < PF; ++k) look_up(at[k], step + k * W);
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const int c = ct * 16 + c16;
@@ -246,21 +247,21 @@ __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
     if (Step::T) qb[ct][KC - 1] = *reinterpret_cast<const bf16x8*>(row + 64 * P + 8 * g);
   }
   __builtin_amdgcn_sched_barrier(0);  // (the queries first, then one step's loads before the next one's: the waits count them)
-  load(a, pa, step);
-  __builtin_amdgcn_sched_barrier(0);
-  load(b, pb, step + W);
-  __builtin_amdgcn_sched_barrier(0);
-  look_up(pa, step + 2 * W);
-  look_up(pb, step + 3 * W);
-  for (; step <= last; step += 2 * W) {  // (no way through the loop leaves out a load)
-    work(a, step);
-    load(a, pa, step + 2 * W);
+#pragma unroll
+  for (int k = 0; k < PF; ++k) {
+    load(s[k], at[k]);
     __builtin_amdgcn_sched_barrier(0);
-    look_up(pa, step + 4 * W);
-    if (step + W <= last) work(b, step + W);
-    load(b, pb, step + 3 * W);
-    __builtin_amdgcn_sched_barrier(0);
-    look_up(pb, step + 5 * W);
+  }
+#pragma unroll
+  for (int k = 0; k < PF; ++k) look_up(at[k], step + (PF + k) * W);
+  for (; step <= last; step += PF * W) {  // (no way through the loop leaves out a load)
+#pragma unroll
+    for (int k = 0; k < PF; ++k) {
+      if (k == 0 || step + k * W <= last) work(s[k], step + k * W);
+      load(s[k], at[k]);
+      __builtin_amdgcn_sched_barrier(0);
+      look_up(at[k], step + (2 * PF + k) * W);
+    }
   }
   bad = __any(bad);
 

@@ -2643,7 +2643,7 @@ class HipOps:
         return out
 
     QUANTIZED_TOKENS = 512  # a segment of more tokens never takes the kernel over codes
-    QUANTIZED_RANGES = 128  # of a (tile, kv head), at most
+    QUANTIZED_RANGES = 64  # of a (tile, kv head), at most
     # measured on MI355X at head size 128, bfloat16 queries.  The kernel over codes: a block of eight wavefronts with up to 16
     # columns works through a key in 4.8 ns (98 to 32,768 keys; with up to 32 columns in 8.9), all blocks together through
     # 6.4 TB/s; a block begins and ends in 3.5 us, ranges that hand each other results cost 3 us and 0.1 us a range.  Pages read
@@ -2653,9 +2653,10 @@ class HipOps:
     QUANTIZED_MERGE_US, QUANTIZED_RESULT_US = 3.0, 0.1
     QUANTIZED_LONG_US, QUANTIZED_LONG_KEY_US, QUANTIZED_LONG_FLOPS_PER_US = 9.0, 0.026, 7.5e8
 
-    def _quantized_split(self, ranges_of, keys_of_all: int, keys_read: int, num_kv_heads: int, head_dim: int, wide: bool):
+    def _quantized_split(self, ranges_of, longest: int, keys_read: int, num_kv_heads: int, head_dim: int, wide: bool):
         """How many keys a range of a (tile, kv head) has.  ``ranges_of(keys)``: how many ranges of so many keys the tiles have,
-        in all and at most; ``keys_of_all``: the tiles' keys, ``keys_read``: the same with those that tiles share counted once.
+        in all and at most; ``longest``: the most keys of a tile, ``keys_read``: all tiles' keys, those that some share counted
+        once.
         Returns ``(microseconds, the most ranges of a tile, keys a range, wavefronts a block)``."""
         best, keys = None, 256
         key_us = self.QUANTIZED_KEY_US * head_dim / 128 * (1.85 if wide else 1.0)
@@ -2664,7 +2665,7 @@ class HipOps:
             blocks, most = ranges_of(keys)
             if most <= self.QUANTIZED_RANGES:
                 rounds = -(-num_kv_heads * blocks // self._compute_units)
-                cost = max(rounds * (self.QUANTIZED_BLOCK_US + min(keys, keys_of_all) * key_us), self.QUANTIZED_BLOCK_US + read_us)
+                cost = max(rounds * (self.QUANTIZED_BLOCK_US + min(keys, longest) * key_us), self.QUANTIZED_BLOCK_US + read_us)
                 if most > 1:
                     cost += self.QUANTIZED_MERGE_US + self.QUANTIZED_RESULT_US * most
                 if best is None or cost < best[0]:
@@ -2702,7 +2703,7 @@ class HipOps:
                 return int(each.sum()), int(each.max())
 
             read = sum(seg_starts[i] + seg_lens[i] - first_needed_position(retention, seg_starts[i]) for i in segments)
-            return tiles, self._quantized_split(ranges_of, int((last - first + 1).sum()), read, num_kv_heads, head_dim, wide)
+            return tiles, self._quantized_split(ranges_of, int((last - first).max()) + 1, read, num_kv_heads, head_dim, wide)
 
         def long_us(segments):
             if not segments:
@@ -2723,7 +2724,7 @@ class HipOps:
                 most = self._most_ranges(retention, decode_bucket, keys)
                 return most * n, most
 
-            split = self._quantized_split(ranges_of, held * n, held * n, num_kv_heads, head_dim, wide)
+            split = self._quantized_split(ranges_of, held, held * n, num_kv_heads, head_dim, wide)
             plan["few"].append((None, n, group, *split[1:], {}))
         else:
             # segments of up to so many tokens go through the kernel over codes: the bound with which the step is done first

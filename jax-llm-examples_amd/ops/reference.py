@@ -669,9 +669,10 @@ class ReferenceOps:
         rot = prep.rotation
         if rot is not None:
             rd = int(rot.rotary_dim) or dh
-            ang = positions.float()[:, None] * rot.inv_freq.float()[None, :]
+            exact = isinstance(kv_cache, QuantizedPages)  # (there an angle is not rounded to float32)
+            ang = positions.to(torch.float64 if exact else torch.float32)[:, None] * rot.inv_freq.float()[None, :]
             grow = float(getattr(rot, "magnitude", 1.0))
-            sin, cos = torch.sin(ang)[:, None, :] * grow, torch.cos(ang)[:, None, :] * grow
+            sin, cos = torch.sin(ang).float()[:, None, :] * grow, torch.cos(ang).float()[:, None, :] * grow
 
             def turn(x):
                 head, rest = x[..., :rd], x[..., rd:]

@@ -246,7 +246,8 @@ class OutputHead(Part):
 class Rotation:
     """A rotary encoding as data: element pairs of a head are turned by ``pos * inv_freq[j]``.
 
-    ``inv_freq``: float32 ``[rotary_dim / 2]``; the angles are formed in float32 inside the kernel.
+    ``inv_freq``: float32 ``[rotary_dim / 2]``; the angles are formed in float32 inside the kernel (for a cache in 8 bits: in
+    float64).
     ``pairing``: ``"adjacent"`` pairs ``(x[2j], x[2j+1])``; ``"half"`` pairs ``(x[j], x[j + rotary_dim/2])``.
     ``rotary_dim``: the leading elements of a head that are rotated (the rest pass unchanged).
     ``magnitude``: a factor on every sine and cosine (the rotated elements grow by it)."""

@@ -187,6 +187,7 @@ SEGS = {
     "portions": [(70, 70), (1, 300), (33, 215), (5, 12), (129, 400)],
     "long": [(1, 9000)],
 }
+SEGS["tens"] = [(17, 17), (40, 900), (1, 333), (100, 2100), (16, 16), (2, 700)]
 HEADS = [(4, 2, 64), (10, 2, 128), (16, 1, 32), (17, 1, 64), (3, 3, 96), (32, 1, 128), (4, 2, 256), (20, 1, 256)]
 
 
@@ -214,7 +215,7 @@ def test_read_pages_gives_every_code_exactly(ops, dh):
 
 
 def _prepared(qkv, hq, hk, dh, pos, prep):
-    """Queries and keys in 64 bits (the angles are float32 products), values."""
+    """Queries and keys in 64 bits, values."""
     x = qkv.double().view(len(pos), -1, dh)
     h, v = x[:, : hq + hk].clone(), x[:, hq + hk:]
     unit = lambda t: t / torch.sqrt((t * t).mean(-1, keepdim=True) + prep.norm_eps)
@@ -225,7 +226,7 @@ def _prepared(qkv, hq, hk, dh, pos, prep):
         h = unit(h) * weights
     r = prep.rotation
     if r is not None:
-        ang = (torch.tensor(pos).float()[:, None] * r.inv_freq[None]).double()[:, None]
+        ang = (torch.tensor(pos).double()[:, None] * r.inv_freq.double()[None])[:, None]
         half = r.rotary_dim // 2
         i = torch.arange(half)
         a, b = (2 * i, 2 * i + 1) if r.pairing == "adjacent" else (i, i + half)
@@ -299,6 +300,28 @@ def test_prepare_writes_rows_in_8_bits(ops, kind, hq, hk, dh, ps):
 
 
 @gpu
+@pytest.mark.parametrize("kind", ["plain", "half", "first"])
+@pytest.mark.parametrize("n", [3, 130])
+def test_prepare_at_far_positions(ops, kind, n):
+    """Positions of millions, where an angle that is a float32 product is off by a tenth and more: keys are the nearest codes
+    of the 64-bit rows but where these lie within 2^-30 of their size of a border."""
+    hq, hk, dh, ps = 4, 2, 128, 16
+    g = _gen(n)
+    pos = (4_000_001 + torch.arange(n) * 100_003).tolist()
+    qkv = torch.randn(n, (hq + 2 * hk) * dh, generator=g).bfloat16()
+    kv = QuantizedPages.empty(-(-n // ps), hk, ps, dh, DEV, poison=True)
+    slots = torch.arange(n, dtype=torch.int32)
+    q = ops.qk_prepare_kv_write(qkv.to(DEV), hq, hk, dh, torch.tensor(pos, dtype=torch.int32, device=DEV), _prep(kind, dh, DEV), kv,
+                                slots.to(DEV)).cpu().double()
+    wq, wk, _ = _prepared(qkv, hq, hk, dh, pos, _prep(kind, dh))
+    assert ((q - wq).abs() <= 2.0 ** -8 * wq.abs() + 64 * 2.0 ** -24 * (wq.abs() + wq.abs().amax(-1, keepdim=True))).all()
+    k, _ = Q.read_rows(QuantizedPages(kv.codes.cpu(), kv.scales.cpu()), torch.arange(kv.shape[0]))
+    k = k.transpose(1, 2).reshape(-1, hk, dh)[:n].double()
+    low, high = held(wk * (1 - 2.0 ** -30))[0], held(wk * (1 + 2.0 ** -30))[0]
+    assert ((k == low) | (k == high)).all()
+
+
+@gpu
 @pytest.mark.parametrize("hq,hk,dh", HEADS)
 @pytest.mark.parametrize("name", list(SEGS))
 def test_attention_over_codes(ops, hq, hk, dh, name):
@@ -308,7 +331,7 @@ def test_attention_over_codes(ops, hq, hk, dh, name):
 
 @gpu
 @pytest.mark.parametrize("rule", [("chunk", 256), ("chunk", 100), ("window", 300), ("window", 1), ("window", 33)], ids=str)
-@pytest.mark.parametrize("name", ["second page", "many", "few", "portions", "long"])
+@pytest.mark.parametrize("name", ["second page", "many", "few", "portions", "long", "tens"])
 def test_attention_over_codes_by_rule(ops, rule, name):
     c = Case(SEGS[name], 10, 2, 128, 16, rule, seed=6)
     c.check(c.run(ops))
@@ -321,6 +344,35 @@ def test_single_tokens_by_page_size_and_layout(ops, ps, single):
     """A step of single tokens laid out for its own lengths, and for the next multiple of the recorded steps' bound."""
     c = Case([(1, t) for t in (1, 15, 16, 17, 2000, 1024, 1025, 511)], 8, 4, 64, ps, seed=7, single=single)
     c.check(c.run(ops))
+
+
+@gpu
+@pytest.mark.parametrize("hq,hk,dh", [(6, 2, 32), (16, 1, 64), (20, 1, 96), (5, 1, 128), (4, 2, 256)])
+@pytest.mark.parametrize("waves", [4, 8])
+def test_every_number_of_ranges_is_joined(ops, hq, hk, dh, waves):
+    """One range to as many as a launch takes, counters that are zero again, and keys beyond what the launch was laid out
+    for: NaN, and nothing waits."""
+    from jax_llm_examples_amd.ops.hip import _p
+
+    c = Case([(1, 4090), (1, 31), (1, 2049)], hq, hk, dh, 16, seed=11)
+    q, n, cols = c.q.to(DEV), 3, hq // hk
+
+    def run(span, ranges):
+        out = torch.empty(n, hq * dh, dtype=torch.bfloat16, device=DEV)
+        ml = torch.empty(n * hk * ranges * cols * 2, device=DEV)
+        wo = torch.empty(n * hk * ranges * cols * dh, device=DEV)
+        tickets = torch.zeros(n * hk, dtype=torch.int32, device=DEV)
+        ops._call("jle_attention_quantized", _p(q), _p(c.kv.codes), _p(c.kv.scales), _p(out), _p(ml), _p(wo), _p(tickets),
+                  _p(c.positions), _p(c.segment), _p(c.table), c.table.shape[1], c.kv.shape[0], None, n, cols, ranges, span,
+                  0, 0, c.scale, hq, hk, dh, 16, waves)
+        assert not tickets.any()
+        return out
+
+    for span in (64, 96, 256, 1024, 2048, 4096):
+        c.check(run(span, -(-4090 // span)))
+    short = run(256, 7).cpu()  # (the second request has one range, the third nine, the first sixteen)
+    want, _ = c.want()
+    assert short[0].isnan().all() and short[2].isnan().all() and not short[1].isnan().any()
 
 
 @gpu
@@ -420,6 +472,37 @@ def test_engine_with_8_bits_gives_the_same_logits_however_prompts_are_cut(model_
         e = _engine(model_dirs_bf16["B"], "cpu", max_num_batched_tokens=budget, poison=True)
         got.append(e.prefill(_prompts(1000))[1])
     assert torch.allclose(got[0], got[1], rtol=1e-4, atol=1e-4)
+
+
+def test_requests_that_lose_their_pages_and_start_again_give_the_same_tokens(model_dirs_bf16):
+    from jax_llm_examples_amd import Engine, SamplingParams, load_model
+
+    got = []
+    for tokens in (1024, 96):  # (96: two of the three requests do not fit at once to their end)
+        e = Engine(load_model(model_dirs_bf16["B"], "bfloat16", "cpu"), cache_tokens=tokens, decode_batch_size=4,
+                   max_num_batched_tokens=32, kv_dtype="float8_e4m3", reference_ops=True, poison=True)
+        got.append(e.generate(_prompts(1000), SamplingParams(max_decode_length=24)))
+        e.cache.check()
+    assert e.scheduler.stats["preemptions"] > 0 and got[0] == got[1]
+
+
+def test_a_replay_holds_its_cache_in_8_bits(model_dirs_bf16, tmp_path):
+    import json
+
+    import numpy as np
+
+    from jax_llm_examples_amd.engine.replay import make_runner, replay
+
+    out = {}
+    for kv in (None, "float8_e4m3"):
+        runner = make_runner(model_dirs_bf16["B"], "bfloat16", 256, "cpu", reference_ops=True, poison=True, kv_dtype=kv)
+        steps = [{"step": 0, "entries": [{"id": "a", "tokens": list(range(30)), "want": [29]}]},
+                 {"step": 1, "entries": [{"id": "a", "tokens": [5], "want": [0]}], "end": ["a"]}]
+        replay(runner, [json.dumps(s) for s in steps], str(tmp_path / str(kv)))
+        assert isinstance(next(iter(runner.cache.groups[0].tensors.values())), QuantizedPages) == (kv is not None)
+        out[kv] = np.fromfile(str(tmp_path / str(kv) / "1.f32"), "<f4")
+    far = np.linalg.norm(out[None] - out["float8_e4m3"]) / np.linalg.norm(out[None])
+    assert 0 < far < 0.1
 
 
 def test_pool_sizes_by_memory_hold_about_twice_the_tokens(model_dirs_bf16):
