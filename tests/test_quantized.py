@@ -400,6 +400,108 @@ def test_missing_pages_give_nan_to_their_queries_alone(ops):
         assert not got[:n].isnan().any() and got[n:].isnan().all()
 
 
+def _from_rows(ops, c, qkv, prep):
+    return ops.attention_from_qkv(qkv, c.hq, c.hk, c.dh, c.positions, c.segment, prep, c.kv, True, c.slots, c.table, c.rule, c.scale,
+                                  c.meta)
+
+
+@gpu
+def test_two_recordings_of_one_plan_replayed_at_once(ops):
+    """Two graphs recorded with the same step's plan, and the same calls launched one by one, on three streams at once: each
+    has counters and results of its own.  Every replay gives the unrecorded call's bits, with other work in between."""
+    cases = [Case([(1, t) for t in (3000, 2500, 17, 4000)], 10, 2, 128, 16, seed=s, single=True) for s in (1, 2, 3)]
+    for c in cases[1:]:
+        c.meta = cases[0].meta  # (the plan asks for lengths and bounds only, which are alike)
+    want = [c.run(ops).clone() for c in cases]
+    (plan,) = cases[0].meta.meta.values()
+    assert plan["few"][0][3] > 1 and plan["tickets"] > 0
+    streams = [torch.cuda.Stream() for _ in cases]
+    qs = [c.q.to(DEV) for c in cases]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for c, q, s in zip(cases[:2], qs, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append([ops.paged_attention(q, c.kv, c.table, c.positions, c.segment, c.rule, c.scale, c.meta) for _ in range(6)])
+        graphs.append(g)
+    for turn in range(5):
+        for o in outs:
+            for x in o:
+                x.fill_(7.0)
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(streams[2]):
+            loose = [ops.paged_attention(qs[2], cases[2].kv, cases[2].table, cases[2].positions, cases[2].segment, cases[2].rule,
+                                         cases[2].scale, cases[2].meta) for _ in range(6)]
+        torch.cuda.synchronize()
+        for got, w in zip([*outs, loose], want):
+            assert all(torch.equal(x, w) for x in got), turn
+        torch.randn(1000, device=DEV).sum().item()
+
+
+@gpu
+def test_a_recorded_layer_writes_and_reads_what_the_next_replay_finds(ops):
+    """From the projected rows, recorded once and replayed with other rows, positions and slots in the same buffers: what an
+    unrecorded call of the same step gives, bit for bit, the pages included."""
+    c = Case([(1, t) for t in (1000, 40, 1023, 333)], 8, 4, 64, 16, seed=4, single=True)
+    prep = _prep("plain", 64, DEV)
+    qkv = (torch.randn(4, 16 * 64, generator=_gen(1)) * 2).bfloat16().to(DEV)
+    before = (c.kv.codes.clone(), c.kv.scales.clone())
+    _from_rows(ops, c, qkv, prep)  # (its plan)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = _from_rows(ops, c, qkv, prep)
+    rows = [(torch.randn(4, 16 * 64, generator=_gen(s)) * 2).bfloat16().to(DEV) for s in (5, 6, 7)]
+    got = []
+    for recorded in (True, False):
+        c.kv.codes.copy_(before[0])
+        c.kv.scales.copy_(before[1])
+        c.positions.copy_(torch.tensor([999, 39, 1022, 332], dtype=torch.int32))
+        mine = []
+        for step, r in enumerate(rows):
+            # (back by a token each step: its slot is the one before)
+            page = c.table.gather(1, (c.positions.long() // 16)[:, None]).squeeze(1)
+            c.slots.copy_(page * 16 + c.positions % 16)
+            qkv.copy_(r)
+            if recorded:
+                g.replay()
+                mine.append(out.clone())
+            else:
+                mine.append(_from_rows(ops, c, qkv, prep))
+            torch.cuda.synchronize()
+            c.positions.sub_(1)
+        got.append((mine, c.kv.codes.clone(), c.kv.scales.clone()))
+    assert all(torch.equal(a, b) for a, b in zip(got[0][0], got[1][0]))
+    assert torch.equal(got[0][1], got[1][1]) and torch.equal(got[0][2], got[1][2])
+
+
+@gpu
+def test_pages_beyond_4_gib(ops):
+    """Codes whose places pass 32 bits: rows written, read back and attended to at the end of a pool of 4.2 GiB."""
+    hq, hk, dh, ps = 8, 8, 128, 16
+    P = 140_000  # of 32 KiB
+    kv = QuantizedPages(torch.zeros(P, hk, 2, ps, dh, dtype=torch.uint8, device=DEV),
+                        torch.full((P, hk, 2, ps), 1, dtype=torch.uint8, device=DEV))
+    n, prep = 40, _prep("plain", dh, DEV)
+    put = lambda x: torch.tensor(list(x), dtype=torch.int32, device=DEV)
+    pages = [P - 1, P - 7, P - 3]
+    qkv = torch.randn(n, (hq + 2 * hk) * dh, generator=_gen(1)).bfloat16().to(DEV)
+    slots = put([pages[i // ps] * ps + i % ps for i in range(n)])
+    q = ops.qk_prepare_kv_write(qkv, hq, hk, dh, put(range(n)), prep, kv, slots)
+    small = QuantizedPages.empty(3, hk, ps, dh, DEV)
+    q2 = ops.qk_prepare_kv_write(qkv, hq, hk, dh, put(range(n)), prep, small, put(range(n)))
+    assert torch.equal(q, q2)
+    assert torch.equal(ops.read_pages(kv, put(pages))[:2], ops.read_pages(small, put([0, 1, 2]))[:2])
+    out = []
+    for pool, table in ((kv, pages), (small, [0, 1, 2])):
+        meta = GroupContext(block_table=put([table]), slot_mapping=slots, width=3, retention=("all",), seg_lens=[n], seg_starts=[0])
+        out.append(ops.paged_attention(q, pool, put([table]), put(range(n)), put([0] * n), ("all",), 0.1, meta))
+    assert torch.equal(*out)
+
+
 @gpu
 def test_refused_on_the_gpu(ops):
     from jax_llm_examples_amd.ops.hip import KernelError
