@@ -377,7 +377,7 @@ __global__ __launch_bounds__(256) void quantized_read_kernel(const uint8_t* __re
       }
     }
     if (!ok) v = u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
-    *reinterpret_cast<u32x4*>(dst + 8 * (size_t)at) = v;
+    __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(dst + 8 * (size_t)at));
   }
 }
 
