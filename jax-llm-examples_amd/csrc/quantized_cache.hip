@@ -173,7 +173,7 @@ __global__ __launch_bounds__(TB > 1 ? TB * 64 * TW : 256, 4) void quantized_prep
       const int u = first + k * step, heads = unit(u, kind, h0);
       raw[k] = u32x4{0u, 0u, 0u, 0u};
       if (u < units && token && sub < heads && in_head)
-        raw[k] = *reinterpret_cast<const u32x4*>(row + ((kind == 0 ? 0 : a.Hq + (kind - 1) * a.Hkv) + h0) * dh + in_unit);
+        raw[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(row + ((kind == 0 ? 0 : a.Hq + (kind - 1) * a.Hkv) + h0) * dh + in_unit));
     }
   };
   const int first0 = TB > 1 ? wave % TW : wave + 4 * blockIdx.y;
@@ -220,10 +220,13 @@ __global__ __launch_bounds__(TB > 1 ? TB * 64 * TW : 256, 4) void quantized_prep
       if (kind == 0) {
         prepare_head<float, LPH>(x, a, a.norm_wq, l, live, turns32 + tk * pairs);
         const float mul = temper[tk];
-        if (live)
-          *reinterpret_cast<u32x4*>(a.q_out + ((size_t)n * a.Hq + h0) * dh + in_unit) =
-              u32x4{pack_bf16(x[0] * mul, x[1] * mul), pack_bf16(x[2] * mul, x[3] * mul), pack_bf16(x[4] * mul, x[5] * mul),
+        if (live) {
+          const u32x4 v = u32x4{pack_bf16(x[0] * mul, x[1] * mul), pack_bf16(x[2] * mul, x[3] * mul), pack_bf16(x[4] * mul, x[5] * mul),
                     pack_bf16(x[6] * mul, x[7] * mul)};
+          u32x4* dst = reinterpret_cast<u32x4*>(a.q_out + ((size_t)n * a.Hq + h0) * dh + in_unit);
+          if (TW == 1 && TB > 1) __builtin_nontemporal_store(v, dst);
+          else *dst = v;
+        }
         continue;
       }
       if (kind == 1) {
