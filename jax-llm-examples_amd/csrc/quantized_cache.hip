@@ -131,8 +131,9 @@ __device__ __forceinline__ void prepare_head(F (&x)[8], const PrepareArgs& a, co
 // LPH lanes a head (a power of two, at least dh / 8), eight neighbouring elements a lane, 64 / LPH heads of a kind (queries,
 // keys, values) a wavefront at a time: a *unit*.  A block takes TB consecutive tokens and forms their sines and cosines once.
 // With one token a block (few tokens) the units are shared out among gridDim.y blocks of four wavefronts and the codes go
-// straight into their pages; with several TW wavefronts share a token, the codes are gathered in shared memory and written
-// in larger pieces: keys eight codes each, the tokens' side by side, values the four keys of four elements in 16 bytes where
+// straight into their pages (one token of 56 heads 4.3 us, 64 of 32 5.2); with several TW wavefronts share a token, the codes
+// are gathered in shared memory and written in larger pieces (8,191 tokens of 48 heads of 128: 48 us, 3.9 TB/s, 98 when every
+// value was stored by itself; vector instructions bound it, 1,850 a token and wavefront): keys eight codes each, the tokens' side by side, values the four keys of four elements in 16 bytes where
 // the block's tokens fill an aligned four of a page (other values byte by byte).
 template <int LPH, int TB, int TW>
 __global__ __launch_bounds__(TB > 1 ? TB * 64 * TW : 256, 4) void quantized_prepare_kernel(PrepareArgs a) {
@@ -321,8 +322,8 @@ __global__ __launch_bounds__(TB > 1 ? TB * 64 * TW : 256, 4) void quantized_prep
 // Pages in bfloat16, in the layout of the attention kernels (keys [page_size][dh], values [dh][page_size]; every number is
 // exact).  Page i is page_ids[where[i]] (where null: page_ids[i]); an id that is no page's gives NaN.  An item is 16 bytes of
 // the result: eight elements of a key, or eight keys of an element of the values; blockIdx: (page, part of its items, keys or
-// values), and a page's items follow each other in the result's order, so that every store of a wavefront is one kilobyte
-// (values of pages of sixteen: with pages of 16 and more tokens a row of theirs, 32 bytes and more).
+// values), and a page's items follow each other in the result's order, so that every store of a wavefront is one kilobyte.
+// Memory bounds it: 32,768 tokens of 8 x 128 31 us, 6.5 TB/s, with stores that the caches need not keep (with others 37 to 46).
 constexpr int kReadItems = 4;  // of a thread
 __device__ __forceinline__ uint32_t two_bf16(uint32_t w, float scale, bool hi) {
   return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true)
