@@ -2578,11 +2578,21 @@ class HipOps:
                 raise KernelError(str(e)) from None
             self._quantized_sizes.add((num_heads, hk, dh, ps))
 
-    def _here(self, t, what: str) -> None:
+    def _here(self, t, what: str, align: int = 16) -> None:
         if t.device != self._tickets.device:
             raise KernelError(f"{what} must be on the GPU that the kernels run on, {self._tickets.device}, not on {t.device}")
-        if t.data_ptr() % 16:
-            raise KernelError(f"{what} must be aligned to 16 bytes")
+        if t.data_ptr() % align:
+            raise KernelError(f"{what} must be aligned to {align} bytes")
+
+    def _lies(self, t, dtype) -> bool:
+        """Whether the kernels over codes take a tensor as it lies in memory."""
+        return (t.dtype is dtype and t.get_device() == self._device_index and t.is_contiguous()
+                and not t.data_ptr() & (15 if dtype is torch.bfloat16 else 3))
+
+    def _fits(self, kv, num_heads: int, num_kv_heads: int, head_dim: int) -> bool:
+        _, _, hk, ps, dh = kv.shape
+        return (hk == num_kv_heads and dh == head_dim and (num_heads, hk, dh, ps) in self._quantized_sizes
+                and kv.codes.get_device() == self._device_index and not kv.codes.data_ptr() & 15)
 
     def _chk16(self, t, dtype, shape, what: str):
         self._chk(t, dtype, shape, what)
@@ -2593,11 +2603,14 @@ class HipOps:
                               writes: bool = True, clear=None):
         n = qkv.shape[0]
         hq, hk, dh = num_heads, num_kv_heads, head_dim
-        self._chk_quantized(kv, hq, hk, dh)
-        self._chk16(qkv, torch.bfloat16, (n, (hq + 2 * hk) * dh), "q|k|v (for a cache in 8 bits)")
-        self._chk(positions, torch.int32, (n,), "positions")
-        if writes:
-            self._chk(slot_mapping, torch.int32, (n,), "slot mapping")
+        if not (self._fits(kv, hq, hk, dh) and self._lies(qkv, torch.bfloat16) and qkv.shape == (n, (hq + 2 * hk) * dh)
+                and self._lies(positions, torch.int32) and positions.shape == (n,)
+                and (not writes or self._lies(slot_mapping, torch.int32) and slot_mapping.shape == (n,))):
+            self._chk_quantized(kv, hq, hk, dh)
+            self._chk16(qkv, torch.bfloat16, (n, (hq + 2 * hk) * dh), "q|k|v (for a cache in 8 bits)")
+            for t, what in ((positions, "positions"), *(((slot_mapping, "slot mapping"),) if writes else ())):
+                self._chk(t, torch.int32, (n,), what)
+                self._here(t, what, 4)
         if prep.norm_span != "head":
             raise KernelError("queries and keys for a cache in 8 bits are normed head by head")
         rot, inv_freq, pairing, rd = prep.rotation, None, 0, 0
@@ -2629,17 +2642,20 @@ class HipOps:
         kernels read pages, ``[n, 2, kv_heads, page_size, head_dim]``; every number is exact.  An id that is no page's gives
         NaN."""
         self._chk(page_ids, torch.int32, (page_ids.numel(),), "page ids")
+        self._here(page_ids, "page ids", 4)
         return self._read_pages(kv, page_ids, None)
 
     def _read_pages(self, kv, page_ids, where):
         """``where``: the places of ``page_ids`` that are meant (all, one after the other)."""
         p, _, hk, ps, dh = kv.shape
-        self._chk_quantized(kv, hk, hk, dh)
+        if not self._fits(kv, hk, hk, dh):
+            self._chk_quantized(kv, hk, hk, dh)
         if p == 0:
             raise KernelError("no pages to read")
         n = page_ids.numel() if where is None else where.numel()
         out = torch.empty(n, 2, hk, ps, dh, dtype=torch.bfloat16, device=kv.device)
-        self._call("jle_quantized_read", _p(kv.codes), _p(kv.scales), _p(page_ids), _p(where), _p(out), n, p, hk, dh, ps)
+        self._call("jle_quantized_read", kv.codes.data_ptr(), kv.scales.data_ptr(), page_ids.data_ptr(), _p(where), out.data_ptr(),
+                   n, p, hk, dh, ps)
         return out
 
     QUANTIZED_TOKENS = 512  # a segment of more tokens never takes the kernel over codes
@@ -2783,14 +2799,19 @@ class HipOps:
         """``tickets``: as many zeros as the plan says, for this call alone."""
         n, hq, dh = q.shape
         p, _, hk, ps, _ = kv.shape
-        self._chk_quantized(kv, hq, hk, dh)
-        self._chk16(q, torch.bfloat16, None, "q (over a cache in 8 bits)")
-        self._chk(block_table, torch.int32, None, "block table")
-        self._chk(positions, torch.int32, (n,), "positions")
-        self._chk(token_segment, torch.int32, (n,), "token segments")
-        if not scale > 0:
-            raise KernelError("attention over a cache in 8 bits takes a positive softmax scale")
-        out = torch.empty(n, hq * dh, dtype=torch.bfloat16, device=q.device)
+        # (what a step of few tokens costs is the host's time: all is looked at in one expression, and by itself for the error)
+        if not (self._fits(kv, hq, hk, dh) and self._lies(q, torch.bfloat16) and self._lies(block_table, torch.int32)
+                and self._lies(positions, torch.int32) and self._lies(token_segment, torch.int32) and scale > 0
+                and positions.shape == (n,) and token_segment.shape == (n,)):
+            self._chk_quantized(kv, hq, hk, dh)
+            self._chk16(q, torch.bfloat16, None, "q (over a cache in 8 bits)")
+            for t, shape, what in ((block_table, None, "block table"), (positions, (n,), "positions"),
+                                   (token_segment, (n,), "token segments")):
+                self._chk(t, torch.int32, shape, what)
+                self._here(t, what, 4)
+            if not scale > 0:
+                raise KernelError("attention over a cache in 8 bits takes a positive softmax scale")
+        out = torch.empty(n, hq * dh, dtype=torch.bfloat16, device=self._tickets.device)
         if n == 0:
             return out
         retention = tuple(retention)
@@ -2819,9 +2840,10 @@ class HipOps:
                     used += num * hk
                 else:
                     mine = held[1].data_ptr()
-            self._call("jle_attention_quantized", _p(q), _p(kv.codes), _p(kv.scales), _p(out), ws_ml, ws_o, mine,
-                       _p(positions), _p(token_segment), _p(block_table), block_table.shape[1], p, _p(tiles), num, cols,
-                       ranges, span, mode, param, float(scale), hq, hk, dh, ps, waves)
+            self._call("jle_attention_quantized", q.data_ptr(), kv.codes.data_ptr(), kv.scales.data_ptr(), out.data_ptr(), ws_ml,
+                       ws_o, mine, positions.data_ptr(), token_segment.data_ptr(), block_table.data_ptr(), block_table.shape[1],
+                       p, None if tiles is None else tiles.data_ptr(), num, cols, ranges, span, mode, param, scale, hq, hk, dh,
+                       ps, waves)
         if plan["long"] is not None:
             tiles, where, table = plan["long"]
             pages = self._read_pages(kv, block_table, where)
