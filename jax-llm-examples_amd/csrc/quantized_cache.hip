@@ -149,7 +149,7 @@ __global__ __launch_bounds__(TB > 1 ? TB * 64 * TW : 256, 4) void quantized_prep
   uint8_t* held = reinterpret_cast<uint8_t*>(turns32 + TB * pairs);  // [2][TB][Hkv][dh], several tokens only
   __shared__ int slot_of[TB], leads[TB];
   __shared__ float temper[TB];
-  __shared__ size_t code_at[TB];  // of head 0's keys of the slot's sixteen
+  __shared__ size_t code_at[TB], scales_at[TB];  // of head 0's keys: the codes of the slot's sixteen, the slot's scale byte
   if (a.num_clear > 0 && blockIdx.y == 0)
     for (int i = blockIdx.x * THREADS + threadIdx.x; i < a.num_clear; i += gridDim.x * THREADS) a.clear[i] = 0;
 
@@ -194,16 +194,16 @@ __global__ __launch_bounds__(TB > 1 ? TB * 64 * TW : 256, 4) void quantized_prep
     const int slot = s >= 0 && s < a.num_slots ? (int)s : -1;
     const int page = slot < 0 ? 0 : slot / a.ps, off = slot < 0 ? 0 : slot - page * a.ps;
     slot_of[threadIdx.x] = slot;
-    code_at[threadIdx.x] = ((size_t)page * a.Hkv * 2 * a.ps + (off & ~15)) * dh;
+    const size_t rows = (size_t)page * a.Hkv * 2 * a.ps;
+    code_at[threadIdx.x] = (rows + (off & ~15)) * dh;
+    scales_at[threadIdx.x] = rows + off;
     temper[threadIdx.x] = a.floor_scale > 0.f && m < a.N
                               ? 1.0f + a.attn_scale * log1pf(floorf(((float)a.positions[m] + 1.0f) / a.floor_scale)) : 1.f;
   }
   __syncthreads();
 
   const int slot = slot_of[tk];
-  const size_t plane_codes = (size_t)a.ps * dh, at = code_at[tk];
-  // (of head 0's keys: the slot's scale byte)
-  const size_t scale_at = at / (uint32_t)dh + (uint32_t)(slot & 15);
+  const size_t plane_codes = (size_t)a.ps * dh, at = code_at[tk], scale_at = scales_at[tk];
   for (int first = first0; token && first < units; first += AHEAD * step) {
     ask(next, first + AHEAD * step);
 #pragma unroll

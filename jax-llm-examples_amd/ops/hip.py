@@ -2730,7 +2730,7 @@ class HipOps:
                      / self.QUANTIZED_LONG_FLOPS_PER_US)
             return self.QUANTIZED_LONG_US + max(serial, flops) + 0.4 * min(serial, flops)
 
-        plan = {"few": [], "long": None}
+        plan = {"few": [], "long": None, "tokens": int(offsets[-1])}
         long = []
         if decode_bucket is not None:  # (single tokens; the same for all steps of so many requests below this bound)
             n = len(seg_lens)
@@ -2782,7 +2782,7 @@ class HipOps:
 
     def _quantized_plan_of(self, meta, token_segment, positions, retention, hq: int, kv, block_table):
         _, _, hk, ps, dh = kv.shape
-        key = ("quantized_plan", retention, hk, hq // hk, dh, ps)
+        key = ("quantized_plan", retention, hk, hq // hk, dh, ps, block_table.shape)
         plan = meta.meta.get(key) if meta is not None else None
         if plan is None:
             if retention[0] == "window_keep":
@@ -2793,6 +2793,8 @@ class HipOps:
             plan = self._quantized_plan(seg_lens, seg_starts, retention, hk, hq // hk, dh, ps, bucket, block_table)
             if meta is not None:
                 meta.meta[key] = plan
+        if plan["tokens"] > positions.shape[0]:
+            raise KernelError(f"the step's segments have {plan['tokens']} tokens, its arrays {positions.shape[0]}")
         return plan
 
     def _attention_quantized(self, q, kv, block_table, positions, token_segment, retention, scale: float, meta, tickets=None):
@@ -2842,8 +2844,8 @@ class HipOps:
                     mine = held[1].data_ptr()
             self._call("jle_attention_quantized", q.data_ptr(), kv.codes.data_ptr(), kv.scales.data_ptr(), out.data_ptr(), ws_ml,
                        ws_o, mine, positions.data_ptr(), token_segment.data_ptr(), block_table.data_ptr(), block_table.shape[1],
-                       p, None if tiles is None else tiles.data_ptr(), num, cols, ranges, span, mode, param, scale, hq, hk, dh,
-                       ps, waves)
+                       p, None if tiles is None else tiles.data_ptr(), num, cols, ranges, span, mode, param, float(scale), hq,
+                       hk, dh, ps, waves)
         if plan["long"] is not None:
             tiles, where, table = plan["long"]
             pages = self._read_pages(kv, block_table, where)

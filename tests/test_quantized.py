@@ -513,6 +513,12 @@ def test_refused_on_the_gpu(ops):
         ops.paged_attention(q, c.kv, *args, ("all",), 0.1, c.meta, cap=3.0)
     with pytest.raises(KernelError, match="sinks"):
         ops.paged_attention(q, c.kv, *args, ("all",), 0.1, c.meta, sink=torch.zeros(4, device=DEV))
+    with pytest.raises(KernelError, match="segments have"):
+        short = GroupContext(block_table=c.table, slot_mapping=c.slots, width=3, retention=("all",), seg_lens=[3], seg_starts=[38])
+        ops.paged_attention(q, c.kv, *args, ("all",), 0.1, short)
+    with pytest.raises(KernelError, match="segments have"):
+        short = GroupContext(block_table=c.table, slot_mapping=c.slots, width=3, retention=("all",), seg_lens=[1] * 3, decode_bucket=1024)
+        ops.paged_attention(q, c.kv, *args, ("all",), 0.1, short)
     with pytest.raises(KernelError, match="rules"):
         ops.paged_attention(q, c.kv, *args, ("window_keep", 8, 2), 0.1, c.meta)
     with pytest.raises(KernelError, match="positive"):
