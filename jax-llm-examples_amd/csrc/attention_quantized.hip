@@ -13,12 +13,14 @@
 // sums and accumulators are float32.  The probabilities times the scales are rounded to bfloat16 (half a step: 2^-8 of each),
 // as they are where pages are bfloat16: the matrix instruction multiplies them by codes that it takes exactly.
 //
-// The pages hold the codes in the lanes' order, so every load of a wavefront is a contiguous kilobyte.  A wavefront has two
-// steps of 32 keys in registers or on their way (steps of 64 keys, or three on their way: the same rate and 0.7 to 2.6 us more
-// of a way in).  Where the launch fills the GPU memory bounds it, 2 * dh + 2 bytes a key and kv head: 64 requests of 6,100 keys on
-// 8 kv heads of 128 135 us, 5.9 TB/s, 128 of 2,048 85 us, 6.4.  Where it does not, a wavefront's instructions do: about 340 a
-// step, 1.2 us with two wavefronts a SIMD; hence blocks of eight wavefronts, and ranges: 32,768 keys of one request 19.7 us (13
-// at a copy's rate), 98 keys 4.6.
+// The pages hold the codes in the lanes' order, so every load of a wavefront is a contiguous kilobyte.  A wavefront holds one
+// step of 32 keys and asks for the next one's keys and values as it is done with this one's: 118 registers at dh 128, two
+// blocks of eight wavefronts a compute unit.  (Two steps in registers, one block a compute unit: 98 keys 4.7 us, not 4.0, eight
+// requests of 2,100 13.3, not 11.8; steps of 64 keys, three steps on their way and sixteen wavefronts a block: no faster.)
+// Where the launch fills the GPU memory bounds it, 2 * dh + 2 bytes a key and kv head: 64 requests of 6,100 keys on 8 kv heads
+// of 128 133 us, 6.0 TB/s, 128 of 2,048 83 us, 6.5.  Where it does not, a wavefront's instructions do: about 340 a step, 1.2 us
+// with two wavefronts a SIMD; hence blocks of eight wavefronts, and ranges: 32,768 keys of one request 18.5 us (13 at a copy's
+// rate).
 //
 // The wavefronts' (maximum, sum, unnormalised O^T) are merged in shared memory; with more than one range a (tile, kv head)
 // the blocks' results go through memory, and the block that takes the last ticket adds them up in the ranges' order.  Which
@@ -73,8 +75,9 @@ constexpr int kMostRanges = 64;  // of a (tile, kv head): their maxima and sums 
 
 static_assert(kMostRanges * sizeof(f32x2) <= 4 * (32 + 4) * sizeof(float), "a column's maxima and sums in its results' place");
 
+// (up to 16 columns and dh 128: two blocks a compute unit; otherwise one)
 template <int DH, int CT, int W>
-__global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
+__global__ __launch_bounds__(W * 64, CT == 1 && DH <= 128 ? 4 : W / 4) void attention_quantized_kernel(
     const bf16_t* q, const uint8_t* codes, const uint8_t* scales,
     bf16_t* __restrict__ out, float* __restrict__ ws_ml, float* __restrict__ ws_o, int* __restrict__ tickets,
     const int* __restrict__ positions, const int* __restrict__ token_segment, const int* __restrict__ block_table,
@@ -111,9 +114,11 @@ __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
   int lo[CT], hi[CT];
   bf16x8 qb[CT][KC];
 
-  // The pages of a step are looked up, through the scalar path, two steps before their data is asked for: no load waits for
-  // the block table.  And every load is issued, whether its keys exist or not (then it reads the range's nearest tile, and what
-  // it brings is masked or not used): the wait for one step's data then never includes the next one's.
+  // The keys of a wavefront's next step are asked for when this step's scores are formed, its values when this step's are added
+  // up: one step's registers, and the loads of both on their way meanwhile.  Their pages are looked up, through the scalar
+  // path, a step before that: no load waits for the block table.  And every load in the loop is issued, whether its keys exist
+  // or not (then it reads the range's nearest tile, and what it brings is masked): the waits count loads, and no way through the
+  // loop may leave one out.  A wavefront's last step asks for nothing and stands behind the loop (98 keys 4.2 -> 4.0 us).
   struct Pages {
     int id[2], off[2];  // per tile of sixteen keys: its page, the place of its first key there
   };
@@ -128,27 +133,38 @@ __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
     }
   };
   const uint32_t page_rows = (uint32_t)Hkv * 2 * ps;
-  auto load = [&](Step& s, const Pages& at) {
+  auto row_of = [&](const Pages& at, int tt) {  // of the tile's first key, among all pages' keys and values
+    const bool ok = (uint32_t)at.id[tt] < (uint32_t)num_pages;
+    bad |= !ok;  // (a page is missing: the result is NaN)
+    return (uint64_t)(uint32_t)(ok ? at.id[tt] : 0) * page_rows + (uint32_t)(hk * 2 * ps + at.off[tt]);
+  };
+  Step s;
+  auto load_keys = [&](const Pages& at) {
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
-      const bool ok = (uint32_t)at.id[tt] < (uint32_t)num_pages;
-      bad |= !ok;  // (a page is missing: the result is NaN)
-      const uint64_t row = (uint64_t)(uint32_t)(ok ? at.id[tt] : 0) * page_rows + (uint32_t)(hk * 2 * ps + at.off[tt]);
+      const uint64_t row = row_of(at, tt);
       const uint8_t* kp = codes + row * DH;
-      const uint8_t* vp = kp + ps * DH;
-      const uint8_t* sp = scales + row;
-      s.ks[tt] = sp[c16];
-      s.vs[tt] = *reinterpret_cast<const uint32_t*>(sp + ps + 4 * g);
+      s.ks[tt] = scales[row + c16];
 #pragma unroll
       for (int p = 0; p < P; ++p) s.k[tt][p] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kp + 1024 * p) + lane);
       if (Step::T) s.kt[tt] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(kp + 1024 * P) + lane);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto load_values = [&](const Pages& at) {
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt) {
+      const uint64_t row = row_of(at, tt) + ps;
+      const uint8_t* vp = codes + row * DH;
+      s.vs[tt] = *reinterpret_cast<const uint32_t*>(scales + row + 4 * g);
 #pragma unroll
       for (int p = 0; p < P; ++p) s.v[tt][p] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vp + 1024 * p) + lane);
       if (Step::T) s.vt[tt] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(vp + 1024 * P) + lane);
     }
+    __builtin_amdgcn_sched_barrier(0);
   };
 
-  auto work = [&](Step& s, int step) {
+  auto work = [&](auto more, int step, const Pages& next) {
     f32x4 st[CT][2];
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
@@ -164,6 +180,8 @@ __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
         for (int ct = 0; ct < CT; ++ct) st[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qb[ct][c], st[ct][tt], 0, 0, 0);
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
+    if (more.value) load_keys(next);
     const bool full = 32 * step >= full_lo && 32 * step + 31 <= full_hi;
     if (!full) {
 #pragma unroll
@@ -235,11 +253,9 @@ __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
 
   const int last = k_hi / 32;
   int step = k_lo / 32 + wave;
-  constexpr int PF = 2;  // steps of a wavefront on their way or worked on (three: no faster, and a longer way in)
-  Step s[PF];
-  Pages at[PF];
-#pragma unroll
-  for (int k = 0; k < PF; ++k) look_up(at[k], step + k * W);
+  Pages next, after;
+  look_up(next, step);
+  look_up(after, step + W);
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const int c = ct * 16 + c16;
@@ -254,23 +270,16 @@ __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
     }
     if (Step::T) qb[ct][KC - 1] = *reinterpret_cast<const bf16x8*>(row + 64 * P + 8 * g);
   }
-  __builtin_amdgcn_sched_barrier(0);  // (the queries first, then one step's loads before the next one's: the waits count them)
-#pragma unroll
-  for (int k = 0; k < PF; ++k) {
-    load(s[k], at[k]);
-    __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_sched_barrier(0);  // (the queries first: the loop's waits count what is asked for behind them)
+  load_keys(next);
+  load_values(next);
+  for (; step + W <= last; step += W) {
+    next = after;
+    look_up(after, step + 2 * W);
+    work(std::true_type(), step, next);
+    load_values(next);
   }
-#pragma unroll
-  for (int k = 0; k < PF; ++k) look_up(at[k], step + (PF + k) * W);
-  for (; step <= last; step += PF * W) {  // (no way through the loop leaves out a load)
-#pragma unroll
-    for (int k = 0; k < PF; ++k) {
-      if (k == 0 || step + k * W <= last) work(s[k], step + k * W);
-      load(s[k], at[k]);
-      __builtin_amdgcn_sched_barrier(0);
-      look_up(at[k], step + (2 * PF + k) * W);
-    }
-  }
+  if (step <= last) work(std::false_type(), step, next);
   bad = __any(bad);
 
   // the wavefronts' results, column by column
@@ -383,18 +392,16 @@ __global__ __launch_bounds__(W * 64, W / 4) void attention_quantized_kernel(
 // tiles: [num_tiles][2] = (first row, tokens), tokens * Hq / Hkv <= max_cols <= 32; every tile's
 // tokens are consecutive positions of one segment.  ranges: the most ranges of `range` positions (a multiple of 32) that a
 // tile reads.  ws_ml: [num_tiles][Hkv][ranges][max_cols][2], ws_o: the same with [dh], tickets: [num_tiles][Hkv], zero before
-// and after; null with one range.  tiles null: tile i is the single token i.  waves: of a block (4 or 8, up to 16 columns; 0:
-// as many as suit).
+// and after; null with one range.  tiles null: tile i is the single token i.
 JLE_API int jle_attention_quantized(const void* q, const void* codes, const void* scales, void* out, float* ws_ml,
                                     float* ws_o, int* tickets, const int* positions, const int* token_segment, const int* block_table,
                                     int table_width, int num_pages, const int* tiles, int num_tiles, int max_cols,
                                     int ranges, int range, int ret_mode, int ret_param, float scale, int Hq, int Hkv,
-                                    int dh, int ps, int waves, hipStream_t s) {
+                                    int dh, int ps, hipStream_t s) {
   if (num_tiles <= 0) return 0;
   if (!quantized_head_ok(dh) || Hkv <= 0 || Hq % Hkv || ps < 16 || ps % 16 || max_cols < Hq / Hkv) return JLE_BAD_ARG;
   if (table_width < 1 || max_cols > 32 || ranges < 1 || range < 32 || range % 32 || num_pages <= 0) return JLE_BAD_ARG;
   if (ranges > 1 && (ws_ml == nullptr || ws_o == nullptr || tickets == nullptr)) return JLE_BAD_ARG;
-  if (waves != 0 && waves != 4 && waves != 8) return JLE_BAD_ARG;
   if ((ret_mode == 1 || ret_mode == 2) && ret_param <= 0) return JLE_BAD_ARG;
   if (((uintptr_t)ws_ml | (uintptr_t)ws_o) & 7) return JLE_BAD_ARG;
   if (!(scale > 0.f) || (((uintptr_t)q | (uintptr_t)codes | (uintptr_t)scales | (uintptr_t)out) & 15)) return JLE_BAD_ARG;
@@ -413,19 +420,15 @@ JLE_API int jle_attention_quantized(const void* q, const void* codes, const void
   } while (0)
 #define PICK(DH)                               \
   do {                                         \
-    if (max_cols <= 16 && waves == 4) LAUNCH(DH, 1, 4); \
-    else if (max_cols <= 16) LAUNCH(DH, 1, 8); \
-    else LAUNCH(DH, 2, (DH) <= 96 ? 8 : 4);    \
+    if (max_cols <= 16) LAUNCH(DH, 1, 8);      \
+    else LAUNCH(DH, 2, (DH) <= 128 ? 8 : 4);   \
   } while (0)
   switch (dh) {
     case 32: PICK(32); break;
     case 64: PICK(64); break;
     case 96: PICK(96); break;
     case 128: PICK(128); break;
-    case 256:
-      if (max_cols <= 16) LAUNCH(256, 1, 4);
-      else LAUNCH(256, 2, 4);
-      break;
+    case 256: PICK(256); break;
   }
 #undef PICK
 #undef LAUNCH

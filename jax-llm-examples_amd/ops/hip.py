@@ -136,7 +136,7 @@ _SIGNATURES = {
                               _i, _vp],
     "jle_quantized_read": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
     "jle_attention_quantized": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _i,
-                                _i, _i, _i, _vp],
+                                _i, _i, _vp],
     "jle_paged_attention_biased": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _i, _i, _i, _i, _i, _i, _i, _i, _vp,
                                    _vp, _vp, _i, _vp, _f, _vp],
 }
@@ -2662,32 +2662,32 @@ class HipOps:
     QUANTIZED_RANGES = 64  # of a (tile, kv head), at most
     # measured on MI355X at head size 128, bfloat16 queries.  The kernel over codes: a block of eight wavefronts with up to 16
     # columns works through a key in 4.8 ns (98 to 32,768 keys; with up to 32 columns in 8.9), all blocks together through
-    # 6.4 TB/s; a block begins and ends in 3.5 us, ranges that hand each other results cost 3 us and 0.1 us a range.  Pages read
-    # back and the attention over pages in bfloat16: 9 us, 26 ns a key of the longest segment (4,096 keys 113 us, 16,384 390),
-    # and 750 TFLOP/s, of which about 0.4 does not overlap
-    QUANTIZED_KEY_US, QUANTIZED_BYTES_PER_US, QUANTIZED_BLOCK_US = 0.0048, 6.4e6, 3.5
-    QUANTIZED_MERGE_US, QUANTIZED_RESULT_US = 3.0, 0.1
+    # 6.4 TB/s, of which about 0.3 of the lesser does not overlap; a block begins and ends in 3.2 us, ranges that hand each other
+    # results cost 2 us and 0.2 us a range (the choice is the fastest of 256 to 32,768 keys a range, or within 4%, for 1 to 128
+    # requests of 98 to 32,768 keys).  Pages read back and the attention over pages in bfloat16: 9 us, 26 ns a key of the
+    # longest segment (4,096 keys 113 us, 16,384 390), and 750 TFLOP/s, of which about 0.4 does not overlap
+    QUANTIZED_KEY_US, QUANTIZED_BYTES_PER_US, QUANTIZED_BLOCK_US = 0.0048, 6.4e6, 3.2
+    QUANTIZED_MERGE_US, QUANTIZED_RESULT_US = 2.0, 0.2
     QUANTIZED_LONG_US, QUANTIZED_LONG_KEY_US, QUANTIZED_LONG_FLOPS_PER_US = 9.0, 0.026, 7.5e8
 
-    def _quantized_split(self, ranges_of, longest: int, keys_read: int, num_kv_heads: int, head_dim: int, wide: bool):
+    def _quantized_split(self, ranges_of, longest: int, total: int, keys_read: int, num_kv_heads: int, head_dim: int, wide: bool):
         """How many keys a range of a (tile, kv head) has.  ``ranges_of(keys)``: how many ranges of so many keys the tiles have,
-        in all and at most; ``longest``: the most keys of a tile, ``keys_read``: all tiles' keys, those that some share counted
-        once.
-        Returns ``(microseconds, the most ranges of a tile, keys a range, wavefronts a block)``."""
-        best, keys = None, 256
+        in all and at most; ``longest``: the most keys of a tile, ``total``: all tiles' keys, ``keys_read``: the same, those that
+        some share counted once.  Returns ``(microseconds, the most ranges of a tile, keys a range)``."""
         key_us = self.QUANTIZED_KEY_US * head_dim / 128 * (1.85 if wide else 1.0)
+        worked = num_kv_heads * total / self._compute_units  # (keys a compute unit)
         read_us = num_kv_heads * keys_read * 2 * _quantized.bytes_per_row(head_dim) / self.QUANTIZED_BYTES_PER_US
+        best, keys = None, 256
         while True:
             blocks, most = ranges_of(keys)
             if most <= self.QUANTIZED_RANGES:
-                rounds = -(-num_kv_heads * blocks // self._compute_units)
-                cost = max(rounds * (self.QUANTIZED_BLOCK_US + min(keys, longest) * key_us), self.QUANTIZED_BLOCK_US + read_us)
+                work_us = max(min(keys, longest), worked) * key_us
+                cost = (self.QUANTIZED_BLOCK_US * max(1.0, num_kv_heads * blocks / self._compute_units)
+                        + max(work_us, read_us) + 0.3 * min(work_us, read_us))
                 if most > 1:
                     cost += self.QUANTIZED_MERGE_US + self.QUANTIZED_RESULT_US * most
                 if best is None or cost < best[0]:
-                    # four rounds of blocks and more: smaller blocks, three of which share a compute unit (128 requests of
-                    # 2,048 keys 92 -> 85 us, 64 of 6,100 135 -> 138)
-                    best = (cost, most, keys, 4 if rounds >= 4 else 8)
+                    best = (cost, most, keys)
                 if most == 1:
                     return best
             keys += 256 if keys < 2048 else keys
@@ -2719,7 +2719,8 @@ class HipOps:
                 return int(each.sum()), int(each.max())
 
             read = sum(seg_starts[i] + seg_lens[i] - first_needed_position(retention, seg_starts[i]) for i in segments)
-            return tiles, self._quantized_split(ranges_of, int((last - first).max()) + 1, read, num_kv_heads, head_dim, wide)
+            each = last - first + 1
+            return tiles, self._quantized_split(ranges_of, int(each.max()), int(each.sum()), read, num_kv_heads, head_dim, wide)
 
         def long_us(segments):
             if not segments:
@@ -2740,7 +2741,7 @@ class HipOps:
                 most = self._most_ranges(retention, decode_bucket, keys)
                 return most * n, most
 
-            split = self._quantized_split(ranges_of, held, held * n, num_kv_heads, head_dim, wide)
+            split = self._quantized_split(ranges_of, held, held * n, held * n, num_kv_heads, head_dim, wide)
             plan["few"].append((None, n, group, *split[1:], {}))
         else:
             # segments of up to so many tokens go through the kernel over codes: the bound with which the step is done first
@@ -2762,7 +2763,7 @@ class HipOps:
                 if len(tiles) != len(seg_lens) or any(n != 1 for n in seg_lens):
                     listed = to_device(torch.from_numpy(np.array([x for at, n, _ in tiles for x in (at, n)], np.int32)), device)
                 plan["few"].append((listed, len(tiles), max(n for _, n, _ in tiles) * group, *split[1:], {}))
-        plan["tickets"] = sum(num * num_kv_heads for _, num, _, ranges, _, _, _ in plan["few"] if ranges > 1)
+        plan["tickets"] = sum(num * num_kv_heads for _, num, _, ranges, _, _ in plan["few"] if ranges > 1)
         if long:
             ps, width = page_size, block_table.shape[1]
             where = []
@@ -2821,7 +2822,7 @@ class HipOps:
         mode = _RET_MODES[retention[0]]
         param = int(retention[1]) if mode else 0
         used = 0
-        for tiles, num, cols, ranges, span, waves, kept in plan["few"]:
+        for tiles, num, cols, ranges, span, kept in plan["few"]:
             ws_ml = ws_o = mine = None
             if ranges > 1:
                 # Counters (zero before and after every launch) and the ranges' results.  A recorded call has its own: two
@@ -2845,7 +2846,7 @@ class HipOps:
             self._call("jle_attention_quantized", q.data_ptr(), kv.codes.data_ptr(), kv.scales.data_ptr(), out.data_ptr(), ws_ml,
                        ws_o, mine, positions.data_ptr(), token_segment.data_ptr(), block_table.data_ptr(), block_table.shape[1],
                        p, None if tiles is None else tiles.data_ptr(), num, cols, ranges, span, mode, param, float(scale), hq,
-                       hk, dh, ps, waves)
+                       hk, dh, ps)
         if plan["long"] is not None:
             tiles, where, table = plan["long"]
             pages = self._read_pages(kv, block_table, where)
