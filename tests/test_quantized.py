@@ -386,6 +386,29 @@ def test_scores_far_apart_and_alike(ops):
 
 
 @gpu
+@pytest.mark.parametrize("rule", [("all",), ("chunk", 24), ("window", 19)], ids=str)
+@pytest.mark.parametrize("hq,hk,dh", [(4, 2, 32), (2, 1, 128), (6, 2, 96), (20, 1, 64)])
+def test_rows_that_are_no_numbers_reach_only_queries_that_see_them(ops, hq, hk, dh, rule):
+    """A key's row that is NaN, another's values: tokens of the same step and tile that do not see them, those before the
+    token and those whose window or chunk it is not in, have their results, the others NaN."""
+    c = Case([(13, 61), (6, 40), (1, 33), (1, 64)], hq, hk, dh, 16, rule, seed=21)
+    for request, at, which in ((0, 55, 1), (0, 30, 0), (1, 36, 0), (1, 38, 1), (2, 32, 1), (3, 20, 1), (3, 44, 1)):
+        page = int(c.cpu[0][request, at // 16])
+        if page < 0:
+            continue
+        where = Q.places(dh)[which][at % 16].to(DEV)
+        c.kv.codes[page, :, which].view(hk, 16 * dh)[:, where] = Q.NAN_CODE
+        c.kv.scales[page, :, which, at % 16] = 127
+        (c.v if which else c.k)[page, :, at % 16] = float("nan")
+    want, tol = c.want()
+    got = c.run(ops).cpu().double()
+    assert want.isnan().any() and not want.isnan().all()
+    assert (got.isnan() == want.isnan()).all()
+    fine = ~want.isnan()
+    assert ((got - want).abs() <= tol)[fine].all()
+
+
+@gpu
 def test_missing_pages_give_nan_to_their_queries_alone(ops):
     for n in (1, 3, 40):
         c = Case([(n, 200), (n, 200)], 4, 2, 64, 16, seed=9)
