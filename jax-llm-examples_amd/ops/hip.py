@@ -2658,23 +2658,36 @@ class HipOps:
                    n, p, hk, dh, ps)
         return out
 
-    QUANTIZED_TOKENS = 512  # a segment of more tokens never takes the kernel over codes
+    QUANTIZED_TOKENS = 4096  # a segment of more tokens never takes the kernel over codes
     QUANTIZED_RANGES = 64  # of a (tile, kv head), at most
-    # measured on MI355X at head size 128, bfloat16 queries.  The kernel over codes: a block of eight wavefronts with up to 16
-    # columns works through a key in 4.8 ns (98 to 32,768 keys; with up to 32 columns in 8.9), all blocks together through
-    # 6.4 TB/s, of which about 0.3 of the lesser does not overlap; a block begins and ends in 3.2 us, ranges that hand each other
-    # results cost 2 us and 0.2 us a range (the choice is the fastest of 256 to 32,768 keys a range, or within 4%, for 1 to 128
-    # requests of 98 to 32,768 keys).  Pages read back and the attention over pages in bfloat16: 9 us, 26 ns a key of the
-    # longest segment (4,096 keys 113 us, 16,384 390), and 750 TFLOP/s, of which about 0.4 does not overlap
-    QUANTIZED_KEY_US, QUANTIZED_BYTES_PER_US, QUANTIZED_BLOCK_US = 0.0048, 6.4e6, 3.2
-    QUANTIZED_MERGE_US, QUANTIZED_RESULT_US = 2.0, 0.2
-    QUANTIZED_LONG_US, QUANTIZED_LONG_KEY_US, QUANTIZED_LONG_FLOPS_PER_US = 9.0, 0.026, 7.5e8
+    # Measured on MI355X, bfloat16 queries.  The kernel over codes: a block of eight wavefronts with up to 16 columns works
+    # through a key in 4.8 ns at head size 128 (98 to 32,768 keys), 1.8, 2.8, 3.8 and 9 at 32, 64, 96 and 256; with up to 32
+    # columns in 1.85 times that; all blocks together through 6.4 TB/s, of which about 0.3 of the lesser does not overlap; a
+    # block begins and ends in 3.2 us, others behind it on its compute unit in 1.8 more, ranges that hand each other results
+    # cost 2 us and 0.2 us a range (the choice is the fastest of 256 to 32,768 keys a range, or within 5%, for 1 to 128 requests
+    # of 98 to 32,768 keys).
+    QUANTIZED_KEY_US, QUANTIZED_STEP_US, QUANTIZED_BYTES_PER_US, QUANTIZED_BLOCK_US = 0.004, 0.0008, 6.4e6, 3.2
+    QUANTIZED_ROUND_US, QUANTIZED_MERGE_US, QUANTIZED_RESULT_US = 1.8, 2.0, 0.2
+    # Pages read back and the attention over pages in bfloat16: 9 us, so much a key of the longest segment (4,096 keys of 128
+    # 113 us, 16,384 390, of 256 1,380), and 750 TFLOP/s at head size 128, 500 at others, of which about 0.4 does not overlap.
+    # So a segment of 1,000 tokens on 2,000 keys takes, read back or as codes, 62 or 35 us with 16 heads of 128 on 8 kv heads,
+    # 196 or 37 with 8 of 256 on one, 71 or 82 with 40 of 128 on 8.
+    QUANTIZED_LONG_US, QUANTIZED_LONG_KEY_US = 9.0, {32: 0.024, 64: 0.033, 96: 0.033, 128: 0.025, 256: 0.084}
+    QUANTIZED_LONG_FLOPS_PER_US, QUANTIZED_LONG_FLOPS_PER_US_OTHER = 7.5e8, 5e8
+
+    @staticmethod
+    def _first_seen(retention, positions):
+        """The first keys that queries at these positions (an array) read."""
+        if retention[0] == "all":
+            return np.zeros_like(positions)
+        span = int(retention[1])
+        return positions // span * span if retention[0] == "chunk" else np.maximum(positions - span + 1, 0)
 
     def _quantized_split(self, ranges_of, longest: int, total: int, keys_read: int, num_kv_heads: int, head_dim: int, wide: bool):
         """How many keys a range of a (tile, kv head) has.  ``ranges_of(keys)``: how many ranges of so many keys the tiles have,
         in all and at most; ``longest``: the most keys of a tile, ``total``: all tiles' keys, ``keys_read``: the same, those that
         some share counted once.  Returns ``(microseconds, the most ranges of a tile, keys a range)``."""
-        key_us = self.QUANTIZED_KEY_US * head_dim / 128 * (1.85 if wide else 1.0)
+        key_us = (self.QUANTIZED_STEP_US + self.QUANTIZED_KEY_US * head_dim / 128) * (1.85 if wide else 1.0)
         worked = num_kv_heads * total / self._compute_units  # (keys a compute unit)
         read_us = num_kv_heads * keys_read * 2 * _quantized.bytes_per_row(head_dim) / self.QUANTIZED_BYTES_PER_US
         best, keys = None, 256
@@ -2682,7 +2695,8 @@ class HipOps:
             blocks, most = ranges_of(keys)
             if most <= self.QUANTIZED_RANGES:
                 work_us = max(min(keys, longest), worked) * key_us
-                cost = (self.QUANTIZED_BLOCK_US * max(1.0, num_kv_heads * blocks / self._compute_units)
+                rounds = num_kv_heads * blocks / self._compute_units
+                cost = (self.QUANTIZED_BLOCK_US + self.QUANTIZED_ROUND_US * max(0.0, rounds - 1)
                         + max(work_us, read_us) + 0.3 * min(work_us, read_us))
                 if most > 1:
                     cost += self.QUANTIZED_MERGE_US + self.QUANTIZED_RESULT_US * most
@@ -2708,27 +2722,32 @@ class HipOps:
         offsets = np.concatenate([[0], np.cumsum(seg_lens)]).astype(np.int64)
 
         def few_of(segments):
-            """Tiles ``(row, tokens, first key, last key)`` of the given segments, and their split."""
-            tiles = [(offsets[i] + t, min(tokens, seg_lens[i] - t), seg_starts[i] + t) for i in segments
-                     for t in range(0, seg_lens[i], tokens)]
-            first = np.array([first_needed_position(retention, s) for _, _, s in tiles])
-            last = np.array([s + n - 1 for _, n, s in tiles])
+            """Tiles ``[n, 2]`` (row, tokens) of the given segments, and their split."""
+            lens, starts = (np.array([x[i] for i in segments], np.int64) for x in (seg_lens, seg_starts))
+            counts = -(-lens // tokens)
+            of = np.repeat(np.arange(len(segments)), counts)
+            t = (np.arange(of.size) - np.repeat(np.cumsum(counts) - counts, counts)) * tokens
+            each = np.minimum(tokens, lens[of] - t)
+            start = starts[of] + t
+            last = start + each - 1
+            first = self._first_seen(retention, start)
 
             def ranges_of(keys):
-                each = last // keys - first // keys + 1
-                return int(each.sum()), int(each.max())
+                ranges = last // keys - first // keys + 1
+                return int(ranges.sum()), int(ranges.max())
 
-            read = sum(seg_starts[i] + seg_lens[i] - first_needed_position(retention, seg_starts[i]) for i in segments)
-            each = last - first + 1
-            return tiles, self._quantized_split(ranges_of, int(each.max()), int(each.sum()), read, num_kv_heads, head_dim, wide)
+            keys = last - first + 1
+            read = int((starts + lens - self._first_seen(retention, starts)).sum())
+            return (np.stack([offsets[segments][of] + t, each], 1),
+                    self._quantized_split(ranges_of, int(keys.max()), int(keys.sum()), read, num_kv_heads, head_dim, wide))
 
         def long_us(segments):
             if not segments:
                 return 0.0
             keys = [seg_starts[i] + seg_lens[i] - first_needed_position(retention, seg_starts[i]) for i in segments]
-            serial = max(keys) * self.QUANTIZED_LONG_KEY_US
+            serial = max(keys) * self.QUANTIZED_LONG_KEY_US[head_dim]
             flops = (4.0 * num_kv_heads * group * head_dim * sum(k * seg_lens[i] for k, i in zip(keys, segments))
-                     / self.QUANTIZED_LONG_FLOPS_PER_US)
+                     / (self.QUANTIZED_LONG_FLOPS_PER_US if head_dim == 128 else self.QUANTIZED_LONG_FLOPS_PER_US_OTHER))
             return self.QUANTIZED_LONG_US + max(serial, flops) + 0.4 * min(serial, flops)
 
         plan = {"few": [], "long": None, "tokens": int(offsets[-1])}
@@ -2755,16 +2774,16 @@ class HipOps:
                 rest = [i for i, n in enumerate(seg_lens) if n > bound]
                 if bound != tokens and sum(-(-seg_lens[i] // tokens) for i in mine) > 65535:
                     continue  # (more tiles than a launch takes)
-                tiles, split = few_of(mine) if mine else ([], (0.0,))
+                tiles, split = few_of(mine) if mine else (None, (0.0,))
                 cost = split[0] + long_us(rest)
                 if best is None or cost < best[0]:
                     best = (cost, tiles, split, rest)
             _, tiles, split, long = best
-            if tiles:
+            if tiles is not None:
                 listed = None  # (tile i is token i)
                 if len(tiles) != len(seg_lens) or any(n != 1 for n in seg_lens):
-                    listed = to_device(torch.from_numpy(np.array([x for at, n, _ in tiles for x in (at, n)], np.int32)), device)
-                plan["few"].append((listed, len(tiles), max(n for _, n, _ in tiles) * group, *split[1:], {}))
+                    listed = to_device(torch.from_numpy(tiles.astype(np.int32)), device)
+                plan["few"].append((listed, len(tiles), int(tiles[:, 1].max()) * group, *split[1:], {}))
         plan["tickets"] = sum(num * num_kv_heads for _, num, _, ranges, _, _ in plan["few"] if ranges > 1)
         if long:
             ps, width = page_size, block_table.shape[1]

@@ -338,6 +338,22 @@ def test_attention_over_codes_by_rule(ops, rule, name):
 
 
 @gpu
+@pytest.mark.parametrize("hq,hk,dh", HEADS + [(10, 2, 128)])
+@pytest.mark.parametrize("name", ["portions", "tens", "portion"])
+def test_either_way_of_a_portion(ops, monkeypatch, hq, hk, dh, name):
+    """Segments of many tokens over the codes, and over pages read back, whatever the rule would choose."""
+    c = Case({**SEGS, "portion": [(300, 1100), (1, 70), (600, 600)]}[name], hq, hk, dh, 16, seed=12)
+    for tokens, over in (("QUANTIZED_TOKENS", 0), ("QUANTIZED_LONG_US", 1e9)):
+        with monkeypatch.context() as m:
+            m.setattr(type(ops), tokens, over)
+            c.meta.meta.clear()
+            got = c.run(ops)
+            plan = next(v for k, v in c.meta.meta.items() if isinstance(k, tuple) and k[0] == "quantized_plan")
+            assert (plan["long"] is not None) == (tokens == "QUANTIZED_TOKENS")
+            c.check(got)
+
+
+@gpu
 @pytest.mark.parametrize("ps", [16, 32, 48, 64, 256])
 @pytest.mark.parametrize("single", [False, True])
 def test_single_tokens_by_page_size_and_layout(ops, ps, single):
