@@ -188,13 +188,12 @@ __global__ __launch_bounds__(W * 64, CT == 1 && DH <= 128 ? 4 : W / 4) void atte
       for (int tt = 0; tt < 2; ++tt) {
         // Values and scales of keys outside the range may never have been written: they are read as zero.  So is a row that is
         // NaN throughout: some columns may not see its key, and those that do have NaN from its score.
-        const uint32_t word = P > 0 ? s.v[tt][0][0] : s.vt[tt][0];
-        const uint32_t none = ((word & kCodesNaN) + 0x01010101u) & 0x80808080u;
+        const uint32_t none = codes_none(P > 0 ? s.v[tt][0][0] : s.vt[tt][0]);
         uint32_t keep = 0u;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = 32 * step + 16 * tt + 4 * g + i;
-          const bool nan = none >> (8 * i + 7) & 1u;
+          const bool nan = none >> (8 * i) & 1u;
           keep |= (key >= k_lo) & (key <= k_hi) & !nan ? 255u << (8 * i) : 0u;
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct) {

@@ -18,6 +18,8 @@
 namespace jle {
 
 constexpr uint32_t kCodesNaN = 0x7f7f7f7fu;  // four codes that are no number
+// of four codes, those that are no number: all bits of their bytes
+__device__ __forceinline__ uint32_t codes_none(uint32_t w) { return ((((w & kCodesNaN) + 0x01010101u) & 0x80808080u) >> 7) * 255u; }
 
 __host__ __device__ __forceinline__ int lane_codes(int d, int dh) { return dh - (d & ~63) >= 64 ? 16 : 8; }
 

@@ -323,6 +323,8 @@ __global__ __launch_bounds__(TB > 1 ? TB * 64 * TW : 256, 4) void quantized_prep
 // exact).  Page i is page_ids[where[i]] (where null: page_ids[i]); an id that is no page's gives NaN.  An item is 16 bytes of
 // the result: eight elements of a key, or eight keys of an element of the values; blockIdx: (page, part of its items, keys or
 // values), and a page's items follow each other in the result's order, so that every store of a wavefront is one kilobyte.
+// attend: for attention, whose tiles share the values of keys that some of their queries do not see (zero times NaN is NaN): a
+// row of values that is NaN is read as zero, and its key as NaN, which a mask takes away from the queries that do not see it.
 // Memory bounds it: 32,768 tokens of 8 x 128 31 us, 6.5 TB/s, with stores that the caches need not keep (with others 37 to 46).
 constexpr int kReadItems = 4;  // of a thread
 __device__ __forceinline__ uint32_t two_bf16(uint32_t w, float scale, bool hi) {
@@ -332,7 +334,7 @@ __device__ __forceinline__ uint32_t two_bf16(uint32_t w, float scale, bool hi) {
 __global__ __launch_bounds__(256) void quantized_read_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                              const int* __restrict__ page_ids,
                                                              const int* __restrict__ where, bf16_t* __restrict__ out,
-                                                             int num_pages, int Hkv, int ps, int dh, Divisor plane_items,
+                                                             int num_pages, int attend, int Hkv, int ps, int dh, Divisor plane_items,
                                                              Divisor row_keys, Divisor row_values) {
   const int i = blockIdx.x, which = blockIdx.z;
   const int page = page_ids[where != nullptr ? where[i] : i];
@@ -344,6 +346,7 @@ __global__ __launch_bounds__(256) void quantized_read_kernel(const uint8_t* __re
   bf16_t* dst = out + ((size_t)i * 2 + which) * Hkv * plane_codes;
   const int first = blockIdx.y * (256 * kReadItems) + threadIdx.x;
   u32x2 c[kReadItems], f[kReadItems];
+  uint32_t value[kReadItems] = {};  // attend: a code of the key's values
 #pragma unroll
   for (int k = 0; k < kReadItems; ++k) {  // everything is asked for before the first item is worked on
     const int at = min(first + 256 * k, items - 1);
@@ -354,6 +357,7 @@ __global__ __launch_bounds__(256) void quantized_read_kernel(const uint8_t* __re
       const int key = over(r, row_keys), d = 8 * (r - key * (int)row_keys.d);
       c[k] = *reinterpret_cast<const u32x2*>(plane + (key & ~15) * dh + key_place(d, key & 15, dh));
       f[k][0] = row_scales[key];
+      if (attend) value[k] = plane[plane_codes + (key & ~15) * dh + value_place(0, key & 15, dh)];
     } else {
       const int d = over(r, row_values), key = 8 * (r - d * (int)row_values.d);
       const uint8_t* p = plane + (key & ~15) * dh + value_place(d, key & 15, dh);
@@ -371,7 +375,12 @@ __global__ __launch_bounds__(256) void quantized_read_kernel(const uint8_t* __re
       const float s = scale_of(f[k][0]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = two_bf16(c[k][j >> 1], s, j & 1);
+      if ((value[k] & 0x7fu) == 0x7fu) v = u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
     } else {
+      if (attend) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) c[k][j] &= ~codes_none(c[k][j]);
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const auto x = (j & 1) ? __builtin_amdgcn_cvt_pk_f32_fp8((int)c[k][j >> 1], true)
@@ -439,7 +448,7 @@ JLE_API int jle_quantized_prepare(const void* qkv, void* q_out, void* codes, voi
 }
 
 JLE_API int jle_quantized_read(const void* codes, const void* scales, const int* page_ids, const int* where, void* out,
-                               int n, int num_pages, int Hkv, int dh, int ps, hipStream_t s) {
+                               int n, int num_pages, int attend, int Hkv, int dh, int ps, hipStream_t s) {
   if (n <= 0) return 0;
   if (!jle_quantized_supported(dh, Hkv, Hkv, ps) || num_pages <= 0) return JLE_BAD_ARG;
   if (((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)out) & 15) return JLE_BAD_ARG;
@@ -447,7 +456,7 @@ JLE_API int jle_quantized_read(const void* codes, const void* scales, const int*
   const long long parts = (items + 256 * kReadItems - 1) / (256 * kReadItems);
   if (parts > 65535) return JLE_BAD_ARG;
   hipLaunchKernelGGL(quantized_read_kernel, dim3(n, (unsigned)parts, 2), dim3(256), 0, s, (const uint8_t*)codes,
-                     (const uint8_t*)scales, page_ids, where, (bf16_t*)out, num_pages, Hkv, ps, dh, divisor(ps * (dh / 8)),
+                     (const uint8_t*)scales, page_ids, where, (bf16_t*)out, num_pages, attend, Hkv, ps, dh, divisor(ps * (dh / 8)),
                      divisor(dh / 8), divisor(ps / 8));
   JLE_LAUNCH_CHECK();
   return 0;

@@ -134,7 +134,7 @@ _SIGNATURES = {
                                  _vp, _vp],
     "jle_quantized_prepare": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _vp, _vp, _i, _i, _f, _f, _i, _i, _i, _i, _i, _i, _vp,
                               _i, _vp],
-    "jle_quantized_read": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
+    "jle_quantized_read": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
     "jle_attention_quantized": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _i,
                                 _i, _i, _vp],
     "jle_paged_attention_biased": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _i, _i, _i, _i, _i, _i, _i, _i, _vp,
@@ -2646,7 +2646,9 @@ class HipOps:
         return self._read_pages(kv, page_ids, None)
 
     def _read_pages(self, kv, page_ids, where):
-        """``where``: the places of ``page_ids`` that are meant (all, one after the other)."""
+        """``where``: the places of ``page_ids`` that are meant, for the attention kernels over bfloat16, whose tiles share the
+        values: a row of values that is NaN is then zeros and its key NaN, which the mask keeps from queries that do not see it
+        (None: all pages, one after the other, as they are)."""
         p, _, hk, ps, dh = kv.shape
         if not self._fits(kv, hk, hk, dh):
             self._chk_quantized(kv, hk, hk, dh)
@@ -2655,7 +2657,7 @@ class HipOps:
         n = page_ids.numel() if where is None else where.numel()
         out = torch.empty(n, 2, hk, ps, dh, dtype=torch.bfloat16, device=kv.device)
         self._call("jle_quantized_read", kv.codes.data_ptr(), kv.scales.data_ptr(), page_ids.data_ptr(), _p(where), out.data_ptr(),
-                   n, p, hk, dh, ps)
+                   n, p, int(where is not None), hk, dh, ps)
         return out
 
     QUANTIZED_TOKENS = 4096  # a segment of more tokens never takes the kernel over codes

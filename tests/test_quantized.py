@@ -403,10 +403,12 @@ def test_scores_far_apart_and_alike(ops):
 
 @gpu
 @pytest.mark.parametrize("rule", [("all",), ("chunk", 24), ("window", 19)], ids=str)
-@pytest.mark.parametrize("hq,hk,dh", [(4, 2, 32), (2, 1, 128), (6, 2, 96), (20, 1, 64)])
-def test_rows_that_are_no_numbers_reach_only_queries_that_see_them(ops, hq, hk, dh, rule):
+@pytest.mark.parametrize("hq,hk,dh", [(4, 2, 32), (2, 1, 128), (6, 2, 96), (20, 1, 64), (8, 1, 256)])
+@pytest.mark.parametrize("long", [False, True])
+def test_rows_that_are_no_numbers_reach_only_queries_that_see_them(ops, monkeypatch, hq, hk, dh, rule, long):
     """A key's row that is NaN, another's values: tokens of the same step and tile that do not see them, those before the
-    token and those whose window or chunk it is not in, have their results, the others NaN."""
+    token and those whose window or chunk it is not in, have their results, the others NaN; over the codes and over pages read back."""
+    monkeypatch.setattr(type(ops), *(("QUANTIZED_TOKENS", 0) if long else ("QUANTIZED_LONG_US", 1e9)))
     c = Case([(13, 61), (6, 40), (1, 33), (1, 64)], hq, hk, dh, 16, rule, seed=21)
     for request, at, which in ((0, 55, 1), (0, 30, 0), (1, 36, 0), (1, 38, 1), (2, 32, 1), (3, 20, 1), (3, 44, 1)):
         page = int(c.cpu[0][request, at // 16])
