@@ -18,7 +18,7 @@
 // blocks of eight wavefronts a compute unit.  (Two steps in registers, one block a compute unit: 98 keys 4.7 us, not 4.0, eight
 // requests of 2,100 13.3, not 11.8; steps of 64 keys, three steps on their way and sixteen wavefronts a block: no faster.)
 // Where the launch fills the GPU memory bounds it, 2 * dh + 2 bytes a key and kv head: 64 requests of 6,100 keys on 8 kv heads
-// of 128 133 us, 6.0 TB/s, 128 of 2,048 83 us, 6.5.  Where it does not, a wavefront's instructions do: about 340 a step, 1.2 us
+// of 128 133 us, 6.0 TB/s, 128 of 2,048 83 us, 6.5.  Where it does not, a wavefront's instructions do: about 300 a step, 1.2 us
 // with two wavefronts a SIMD; hence blocks of eight wavefronts, and ranges: 32,768 keys of one request 18.5 us (13 at a copy's
 // rate).
 //
