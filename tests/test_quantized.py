@@ -446,6 +446,25 @@ def _from_rows(ops, c, qkv, prep):
 
 
 @gpu
+def test_two_streams_with_one_plan_at_once(ops):
+    """Calls that may run side by side on two streams, over ranges that are joined: each stream has its own counters and results."""
+    c = Case([(1, 9000), (1, 4000), (3, 2500)], 16, 2, 128, 16, seed=14)
+    alone = c.run(ops)
+    c.check(alone)
+    plan = next(v for k, v in c.meta.meta.items() if isinstance(k, tuple) and k[0] == "quantized_plan")
+    assert any(ranges > 1 for _, _, _, ranges, _, _ in plan["few"])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(c.run(ops))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, alone) for x in got)
+
+
+@gpu
 def test_two_recordings_of_one_plan_replayed_at_once(ops):
     """Two graphs recorded with the same step's plan, and the same calls launched one by one, on three streams at once: each
     has counters and results of its own.  Every replay gives the unrecorded call's bits, with other work in between."""
