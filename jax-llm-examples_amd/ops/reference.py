@@ -739,8 +739,10 @@ class ReferenceOps:
     def attention_from_qkv(self, qkv, num_heads, num_kv_heads, head_dim, positions, token_segment, prep, kv_cache,
                            writes: bool, slot_mapping, block_table, retention, scale: float, meta=None):
         """q and k prepared, k and v written (if this run writes its cache), attention over the pages."""
-        q = self.qk_prepare_kv_write(qkv, num_heads, num_kv_heads, head_dim, positions, prep,
-                                     kv_cache if writes else None, slot_mapping)
+        pages = kv_cache if writes else None
+        if not writes and isinstance(kv_cache, QuantizedPages):  # (the angles of its keys, and no place for these)
+            pages, slot_mapping = kv_cache, torch.full_like(positions, -1)
+        q = self.qk_prepare_kv_write(qkv, num_heads, num_kv_heads, head_dim, positions, prep, pages, slot_mapping)
         return self.paged_attention(q, kv_cache, block_table, positions, token_segment, retention, scale, meta)
 
     def paged_attention(self, q, kv_cache, block_table, positions, token_segment, retention, scale: float, meta=None,

@@ -771,3 +771,33 @@ def test_a_layer_from_its_rows_writes_reads_and_attends(ops):
         # (the queries, as a step that writes nothing prepares them)
         q = ops.qk_prepare_kv_write(qkv, hq, hk, dh, put(pos), prep, kv, torch.full_like(slots, -1)).cpu()
         c.check(got, q)
+
+
+# ------------------------------------------------------------------------------------------------ a run that writes nothing
+@pytest.mark.parametrize("device", ["cpu", pytest.param(DEV, marks=gpu)])
+def test_queries_of_a_run_that_writes_nothing_are_turned_as_the_keys_are(device):
+    """A run that shares another's cache attends to keys at positions in the millions with queries that those angles turned (a
+    float32 product is off by a tenth there and more): the queries are those of a run that writes, and nothing is written."""
+    if device == "cpu":
+        ops = ReferenceOps()
+    else:
+        from jax_llm_examples_amd.engine import get_ops
+        ops = get_ops(device)
+    hq, hk, dh, ps, n = 4, 2, 64, 16, 3
+    c = Case([(n, 40)], hq, hk, dh, ps, ("chunk", 64), seed=31, device=device)
+    base = 64 * 62_501  # (a chunk's beginning: the pages in front of it were given back)
+    table = torch.full((1, (base + 48) // ps), -1, dtype=torch.int32)
+    table[0, base // ps:] = c.cpu[0][0]
+    pos = [base + p for p in c.cpu[1]]
+    positions, table = torch.tensor(pos, dtype=torch.int32, device=device), table.to(device)
+    meta = GroupContext(block_table=table, slot_mapping=c.slots, width=table.shape[1], retention=c.rule, seg_lens=[n], seg_starts=[pos[0]])
+    qkv = torch.randn(n, (hq + 2 * hk) * dh, generator=_gen(2)).bfloat16()
+    prep, rows = _prep("plain", dh, device), qkv.to(device)
+    before = (c.kv.codes.clone(), c.kv.scales.clone())
+    got = ops.attention_from_qkv(rows, hq, hk, dh, positions, c.segment, prep, c.kv, False, c.slots, table, c.rule, c.scale, meta)
+    q = ops.qk_prepare_kv_write(rows, hq, hk, dh, positions, prep, c.kv, torch.full_like(positions, -1))
+    assert torch.equal(c.kv.codes, before[0]) and torch.equal(c.kv.scales, before[1])
+    want = _prepared(qkv, hq, hk, dh, pos, _prep("plain", dh))[0]
+    # (rounded to bfloat16, behind 64 roundings in float32: see the test of prepared rows)
+    assert ((q.cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 64 * 2.0 ** -24 * (want.abs() + want.abs().amax(-1, keepdim=True))).all()
+    assert torch.equal(got, ops.paged_attention(q, c.kv, table, positions, c.segment, c.rule, c.scale, meta))
