@@ -12,7 +12,7 @@ typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
 
 // Keys are normed, turned and scaled in 64 bits (the matrix cores' rate aside, this card adds and multiplies doubles as fast as
 // floats): a code is a rounding to four bits, and where the number to be rounded is itself off by float32's rounding, one code
-// in some hundred thousand falls the other way.  Queries, which are rounded to bfloat16, are worked on in float32, with the
+// in some hundred thousand falls the other way.  The code is the only rounding behind that (toward_odd).  Queries, which are rounded to bfloat16, are worked on in float32, with the
 // same angles.
 
 // Sine and cosine of pos * freq in 64 bits: reduced by multiples of pi / 2 (the product and the remainder by fused
@@ -44,6 +44,17 @@ __device__ __forceinline__ void turn_of(int pos, float freq, double& sn, double&
   const int quarter = (int)((long long)k & 3);
   sn = quarter == 0 ? s : quarter == 1 ? c : quarter == 2 ? -s : -c;
   cs = quarter == 0 ? c : quarter == 1 ? -s : quarter == 2 ? -c : s;
+}
+
+// A 64-bit number on its way to a code, in float32 without a rounding that the code's could follow the wrong way: its fraction
+// is cut behind the 12th bit, which is set where anything but zeros goes (rounding to odd).  So the number stays on its side of
+// every number of fewer bits: of the borders between codes, and of 448 times a power of two, which the scale asks for.  (Twelve,
+// not the 23 of float32: a float below 2^-126 has fewer, and down to a code's smallest half step, 2^-136, it has thirteen.)
+__device__ __forceinline__ float toward_odd(double y) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, y);
+  uint32_t hi = (uint32_t)(b >> 32);
+  hi = (hi & ~0xffu) | min((hi & 0xffu) | (uint32_t)b, 1u) << 8;
+  return (float)__builtin_bit_cast(double, (uint64_t)hi << 32);
 }
 
 struct PrepareArgs {
@@ -236,7 +247,7 @@ __global__ __launch_bounds__(TB > 1 ? TB * 64 * TW : 256, 4) void quantized_prep
         for (int i = 0; i < 8; ++i) y[i] = x[i];
         prepare_head<double, LPH>(y, a, a.norm_wk, l, live, turns + tk * pairs);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (float)y[i];
+        for (int i = 0; i < 8; ++i) x[i] = toward_odd(y[i]);
       }
       uint32_t top = 0;  // the row's largest magnitude, as bits (what is no number is beyond all)
 #pragma unroll

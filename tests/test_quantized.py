@@ -801,3 +801,41 @@ def test_queries_of_a_run_that_writes_nothing_are_turned_as_the_keys_are(device)
     # (rounded to bfloat16, behind 64 roundings in float32: see the test of prepared rows)
     assert ((q.cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 64 * 2.0 ** -24 * (want.abs() + want.abs().amax(-1, keepdim=True))).all()
     assert torch.equal(got, ops.paged_attention(q, c.kv, table, positions, c.segment, c.rule, c.scale, meta))
+
+
+# ------------------------------------------------------------------------------------------------ keys at the codes' borders
+@gpu
+@pytest.mark.parametrize("n", [1, 130])
+@pytest.mark.parametrize("side", [-1, 0, 1])
+def test_keys_that_float32_puts_on_a_border_are_rounded_once(ops, n, side):
+    """Keys whose 64-bit numbers lie beside the border of two codes by less than float32 tells: the nearest code, not the even
+    one.  ``side``: the row's largest magnitude lies as near to 448, below it or beyond it (another scale), or elsewhere (0)."""
+    dh, hq, hk = 128, 2, 1
+    for seed in range(1000):  # (until the largest magnitude lies on the asked side)
+        g = _gen(seed)
+        x = torch.randn(3 + hk, dh, generator=g).bfloat16()
+        k = x[hq].double()
+        k[k == 0] = 1.0
+        x[hq] = k.bfloat16()
+        border = (1 + (2 * torch.randint(0, 8, (dh,), generator=g) + 1) / 16).double() * torch.exp2(torch.randint(-5, 7, (dh,), generator=g).double())
+        border[0] = 448.0 if side else 300.0
+        inv = 1 / torch.sqrt((k * k).mean() + 1e-5)
+        weight = (border / (k * inv).abs()).float()  # (a float32 step of the weight moves a key by up to 2^-23 of it)
+        y = _prepared(x.view(1, -1), hq, hk, dh, [0], QKPreparation(norm_eps=1e-5, norm_weight_q=weight, norm_weight_k=weight))[1]
+        off = (y.abs() / border - 1).view(-1)
+        if side == 0 or (off[0] * side > 2.0 ** -45 and float(y.view(-1)[0].abs().float()) == 448.0):
+            break
+    else:
+        raise AssertionError("no such row")
+    clear = off.abs() > 2.0 ** -45  # (64-bit roundings are 2^-53 of the number, a dozen of them)
+    assert int((clear & (y.view(-1).float().abs().double() == border)).sum()) > dh // 4
+    want, e = held(y)
+    assert float(e) == {-1: 0.0, 0: 0.0, 1: 1.0}[side]
+    device = weight.to(DEV)
+    kv = QuantizedPages.empty(-(-n // 16), hk, 16, dh, DEV, poison=True)
+    rows = x.view(1, -1).expand(n, -1).contiguous().to(DEV)
+    at = torch.arange(n, dtype=torch.int32, device=DEV)
+    ops.qk_prepare_kv_write(rows, hq, hk, dh, at, QKPreparation(norm_eps=1e-5, norm_weight_q=device, norm_weight_k=device), kv, at)
+    got = Q.read_rows(QuantizedPages(kv.codes.cpu(), kv.scales.cpu()), torch.arange(kv.shape[0]))[0]
+    got = got.transpose(1, 2).reshape(-1, hk, dh)[:n].double()
+    assert ((got == want) | ~clear).all()
