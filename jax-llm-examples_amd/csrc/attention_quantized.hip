@@ -399,7 +399,8 @@ __global__ __launch_bounds__(W * 64, CT == 1 && DH <= 128 ? 4 : W / 4) void atte
 // tiles: [num_tiles][2] = (first row, tokens), tokens * Hq / Hkv <= max_cols <= 32; every tile's
 // tokens are consecutive positions of one segment.  ranges: the most ranges of `range` positions (a multiple of 32) that a
 // tile reads.  ws_ml: [num_tiles][Hkv][ranges][max_cols][2], ws_o: the same with [dh], tickets: [num_tiles][Hkv], zero before
-// and after; null with one range.  tiles null: tile i is the single token i.
+// and after; null with one range.  tiles null: tile i is the single token i.  More tiles than kMostTiles: several launches.
+constexpr int kMostTiles = 65535;  // of a launch: the grid's second dimension
 JLE_API int jle_attention_quantized(const void* q, const void* codes, const void* scales, void* out, float* ws_ml,
                                     float* ws_o, int* tickets, const int* positions, const int* token_segment, const int* block_table,
                                     int table_width, int num_pages, const int* tiles, int num_tiles, int max_cols,
@@ -412,7 +413,7 @@ JLE_API int jle_attention_quantized(const void* q, const void* codes, const void
   if ((ret_mode == 1 || ret_mode == 2) && ret_param <= 0) return JLE_BAD_ARG;
   if (((uintptr_t)ws_ml | (uintptr_t)ws_o) & 7) return JLE_BAD_ARG;
   if (!(scale > 0.f) || (((uintptr_t)q | (uintptr_t)codes | (uintptr_t)scales | (uintptr_t)out) & 15)) return JLE_BAD_ARG;
-  if (num_tiles > 65535 || ranges > kMostRanges) return JLE_BAD_ARG;
+  if (ranges > kMostRanges) return JLE_BAD_ARG;
   const float sl = scale * kLog2e;
   const Rule rule = {ret_mode, divisor(ret_mode == 0 ? 1 : ret_param)};
 #define LAUNCH(DH, CT, W)                                                                                                   \
@@ -420,9 +421,11 @@ JLE_API int jle_attention_quantized(const void* q, const void* codes, const void
     const size_t lds = (size_t)(W) * max_cols * ((DH) + 4 + 2) * sizeof(float);                                             \
     const int rc = lds > 64 * 1024 ? allow_lds(attention_quantized_kernel<DH, CT, W>, lds) : 0;                             \
     if (rc) return rc;                                                                                                      \
-    hipLaunchKernelGGL((attention_quantized_kernel<DH, CT, W>), dim3(Hkv, num_tiles, ranges), dim3((W) * 64), lds, s,             \
-                       (const bf16_t*)q, (const uint8_t*)codes, (const uint8_t*)scales, (bf16_t*)out, ws_ml, ws_o, tickets, \
-                       positions, token_segment, block_table, table_width, num_pages, tiles, ranges, divisor(range), rule, sl, Hq, Hkv,    \
+    hipLaunchKernelGGL((attention_quantized_kernel<DH, CT, W>), dim3(Hkv, num, ranges), dim3((W) * 64), lds, s,             \
+                       (const bf16_t*)q + row * Hq * (DH), (const uint8_t*)codes, (const uint8_t*)scales,                   \
+                       (bf16_t*)out + row * Hq * (DH), ws_ml + 2 * slot, ws_o + slot * (DH), tickets + counter,             \
+                       positions + row, token_segment + row, block_table, table_width, num_pages,                           \
+                       tiles == nullptr ? nullptr : tiles + 2 * (size_t)t0, ranges, divisor(range), rule, sl, Hq, Hkv,      \
                        divisor(Hq / Hkv), divisor(ps / 16), max_cols);                                                      \
   } while (0)
 #define PICK(DH)                               \
@@ -430,12 +433,17 @@ JLE_API int jle_attention_quantized(const void* q, const void* codes, const void
     if (max_cols <= 16) LAUNCH(DH, 1, 8);      \
     else LAUNCH(DH, 2, (DH) <= 128 ? 8 : 4);   \
   } while (0)
-  switch (dh) {
-    case 32: PICK(32); break;
-    case 64: PICK(64); break;
-    case 96: PICK(96); break;
-    case 128: PICK(128); break;
-    case 256: PICK(256); break;
+  for (int t0 = 0, num; t0 < num_tiles; t0 += num) {
+    num = num_tiles - t0 < kMostTiles ? num_tiles - t0 : kMostTiles;
+    const size_t row = tiles == nullptr ? t0 : 0;  // (listed tiles name their rows among all)
+    const size_t counter = ranges > 1 ? (size_t)t0 * Hkv : 0, slot = counter * ranges * max_cols;
+    switch (dh) {
+      case 32: PICK(32); break;
+      case 64: PICK(64); break;
+      case 96: PICK(96); break;
+      case 128: PICK(128); break;
+      case 256: PICK(256); break;
+    }
   }
 #undef PICK
 #undef LAUNCH

@@ -2774,8 +2774,6 @@ class HipOps:
             for bound in [tokens, *lengths]:
                 mine = short if bound == tokens else [i for i, n in enumerate(seg_lens) if n <= bound]
                 rest = [i for i, n in enumerate(seg_lens) if n > bound]
-                if bound != tokens and sum(-(-seg_lens[i] // tokens) for i in mine) > 65535:
-                    continue  # (more tiles than a launch takes)
                 tiles, split = few_of(mine) if mine else (None, (0.0,))
                 cost = split[0] + long_us(rest)
                 if best is None or cost < best[0]:

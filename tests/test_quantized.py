@@ -839,3 +839,38 @@ def test_keys_that_float32_puts_on_a_border_are_rounded_once(ops, n, side):
     got = Q.read_rows(QuantizedPages(kv.codes.cpu(), kv.scales.cpu()), torch.arange(kv.shape[0]))[0]
     got = got.transpose(1, 2).reshape(-1, hk, dh)[:n].double()
     assert ((got == want) | ~clear).all()
+
+
+# ------------------------------------------------------------------------------------------------ more tiles than a launch takes
+@gpu
+@pytest.mark.parametrize("kind", ["single", "bucket", "listed", "ranges"])
+def test_more_tiles_than_one_launch_takes(ops, kind):
+    """Sixteen requests 4,200 times over, a tile each: more than a grid's second dimension counts.  Single tokens, laid out for
+    their own lengths or for a bound; beside segments of two tokens, where tiles are listed; in ranges that are joined.  The
+    first sixteen against 64 bits, and all others like them bit for bit."""
+    from jax_llm_examples_amd.ops.hip import _p
+
+    many, hq, hk, dh = 4200, 2, 1, 32
+    segs = [(1, t) for t in (300, 1, 17, 64, 555, 600, 33, 2, 16, 480, 31, 32, 99, 257, 256, 512)]
+    if kind == "listed":
+        segs[3] = (2, 64)
+    c = Case(segs, hq, hk, dh, 16, seed=43, single=kind == "bucket")
+    n, m = c.positions.numel(), c.meta
+    again = lambda x: x.repeat(many, *[1] * (x.dim() - 1))
+    q, positions, table = again(c.q.to(DEV)), again(c.positions), again(c.table)
+    segment = (again(c.segment).view(many, n) + 16 * torch.arange(many, dtype=torch.int32, device=DEV)[:, None]).view(-1)
+    meta = GroupContext(block_table=table, slot_mapping=again(c.slots), width=m.width, retention=c.rule, seg_lens=m.seg_lens * many,
+                        seg_starts=m.seg_starts * many, decode_bucket=m.decode_bucket)
+    if kind == "ranges":
+        out = torch.empty(many * n, hq * dh, dtype=torch.bfloat16, device=DEV)
+        ml, wo = torch.empty(many * 16 * 3 * 2 * 2, device=DEV), torch.empty(many * 16 * 3 * 2 * dh, device=DEV)
+        tickets = torch.zeros(many * 16, dtype=torch.int32, device=DEV)
+        ops._call("jle_attention_quantized", _p(q), _p(c.kv.codes), _p(c.kv.scales), _p(out), _p(ml), _p(wo), _p(tickets), _p(positions),
+                  _p(segment), _p(table), table.shape[1], c.kv.shape[0], None, many * 16, 2, 3, 256, 0, 0, c.scale, hq, hk, dh, 16)
+        assert not tickets.any()
+    else:
+        out = ops.paged_attention(q, c.kv, table, positions, segment, c.rule, c.scale, meta)
+        plan = next(v for k, v in meta.meta.items() if isinstance(k, tuple) and k[0] == "quantized_plan")
+        assert plan["long"] is None and plan["few"][0][1] == 16 * many > 65535
+    c.check(out[:n])
+    assert torch.equal(out, out[:n].repeat(many, 1))
