@@ -2766,13 +2766,13 @@ class HipOps:
             plan["few"].append((None, n, group, *split[1:], {}))
         else:
             # segments of up to so many tokens go through the kernel over codes: the bound with which the step is done first
-            short = [i for i, n in enumerate(seg_lens) if n <= tokens]
+            short = [i for i, n in enumerate(seg_lens) if 0 < n <= tokens]
             lengths = sorted({n for n in seg_lens if tokens < n <= self.QUANTIZED_TOKENS})
             if len(lengths) > 6:
                 lengths = lengths[:: -(-len(lengths) // 6)] + lengths[-1:]
             best = None
             for bound in [tokens, *lengths]:
-                mine = short if bound == tokens else [i for i, n in enumerate(seg_lens) if n <= bound]
+                mine = short if bound == tokens else [i for i, n in enumerate(seg_lens) if 0 < n <= bound]
                 rest = [i for i, n in enumerate(seg_lens) if n > bound]
                 tiles, split = few_of(mine) if mine else (None, (0.0,))
                 cost = split[0] + long_us(rest)

@@ -874,3 +874,38 @@ def test_more_tiles_than_one_launch_takes(ops, kind):
         assert plan["long"] is None and plan["few"][0][1] == 16 * many > 65535
     c.check(out[:n])
     assert torch.equal(out, out[:n].repeat(many, 1))
+
+
+# ------------------------------------------------------------------------------------------------ plans
+def _planner(compute_units=256):
+    """What plans steps, without a GPU."""
+    from jax_llm_examples_amd.ops.hip import HipOps
+
+    ops = HipOps.__new__(HipOps)
+    ops._compute_units, ops._query = compute_units, lambda name, *a: 8
+    return ops
+
+
+@pytest.mark.parametrize("lens", [[0], [0, 0], [0, 300], [300, 0, 0], [0, 1], [0, 5000], [0, 5000, 1, 0, 40]], ids=str)
+@pytest.mark.parametrize("rule", [("all",), ("chunk", 64), ("window", 100)], ids=str)
+def test_segments_of_no_tokens_are_no_work(lens, rule):
+    there = [i for i, n in enumerate(lens) if n]
+    starts = [7 * i + 3 for i in range(len(lens))]
+    table = lambda rows: torch.zeros(rows, 400, dtype=torch.int32)
+    plan = _planner()._quantized_plan(lens, starts, rule, 2, 2, 128, 16, None, table(len(lens)))
+    assert plan["tokens"] == sum(lens)
+    alone = _planner()._quantized_plan([lens[i] for i in there], [starts[i] for i in there], rule, 2, 2, 128, 16, None,
+                                       table(len(there))) if there else {"few": [], "long": None}
+    assert [x[1:5] for x in plan["few"]] == [x[1:5] for x in alone["few"]] and (plan["long"] is None) == (alone["long"] is None)
+
+
+@gpu
+@pytest.mark.parametrize("long", [False, True])
+def test_attention_beside_segments_of_no_tokens(ops, monkeypatch, long):
+    monkeypatch.setattr(type(ops), *(("QUANTIZED_TOKENS", 0) if long else ("QUANTIZED_LONG_US", 1e9)))
+    c = Case([(300, 1100), (1, 70)], 4, 2, 64, 16, seed=51)
+    c.table = c.table[[0, 0, 0, 1, 1]].contiguous()
+    c.segment = (2 * c.segment + 1).contiguous()
+    c.meta = GroupContext(block_table=c.table, slot_mapping=c.slots, width=c.meta.width, retention=c.rule, seg_lens=[0, 300, 0, 1, 0],
+                          seg_starts=[5, 800, 0, 69, 3])
+    c.check(c.run(ops))
