@@ -92,7 +92,14 @@ __global__ __launch_bounds__(W * 64, CT == 1 && DH <= 128 ? 4 : W / 4) void atte
   const int ps = 16 * (int)page_tiles.d, G = (int)group.d;
   const int n0 = tiles != nullptr ? tiles[2 * tile] : tile, nt = tiles != nullptr ? tiles[2 * tile + 1] : 1;
   const int p_first = positions[n0], p_last = p_first + nt - 1;
-  const int first = rule.first(p_first);
+  if (p_last < 0) {  // rows at no position (a batch filled up with such) see no keys: nothing of theirs is looked up
+    for (int i = threadIdx.x; rng == 0 && i < nt * G * (DH / 4); i += W * 64) {
+      const int c = i / (DH / 4), t = over(c, group);
+      *reinterpret_cast<u32x2*>(out + ((size_t)(n0 + t) * Hq + hk * G + c - t * G) * DH + 4 * (i - c * (DH / 4))) = u32x2{0u, 0u};
+    }
+    return;
+  }
+  const int first = rule.first(max(p_first, 0));
   const int r_first = over(first, range), r_abs = r_first + rng;
   const int all_ranges = over(p_last, range) - r_first + 1, mine = min(all_ranges, ranges);
   if (rng >= mine) return;  // (this tile has fewer ranges)

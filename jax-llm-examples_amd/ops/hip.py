@@ -2730,8 +2730,8 @@ class HipOps:
             of = np.repeat(np.arange(len(segments)), counts)
             t = (np.arange(of.size) - np.repeat(np.cumsum(counts) - counts, counts)) * tokens
             each = np.minimum(tokens, lens[of] - t)
-            start = starts[of] + t
-            last = start + each - 1
+            start = np.maximum(starts[of] + t, 0)  # (rows at no position, -1, see no keys)
+            last = np.maximum(starts[of] + t + each - 1, 0)
             first = self._first_seen(retention, start)
 
             def ranges_of(keys):
@@ -2739,7 +2739,7 @@ class HipOps:
                 return int(ranges.sum()), int(ranges.max())
 
             keys = last - first + 1
-            read = int((starts + lens - self._first_seen(retention, starts)).sum())
+            read = int((starts + lens - self._first_seen(retention, np.maximum(starts, 0))).sum())
             return (np.stack([offsets[segments][of] + t, each], 1),
                     self._quantized_split(ranges_of, int(keys.max()), int(keys.sum()), read, num_kv_heads, head_dim, wide))
 
@@ -2789,7 +2789,7 @@ class HipOps:
             ps, width = page_size, block_table.shape[1]
             where = []
             for i in long:
-                first = first_needed_position(retention, seg_starts[i]) // ps
+                first = first_needed_position(retention, max(seg_starts[i], 0)) // ps
                 last = min((seg_starts[i] + seg_lens[i] - 1) // ps, width - 1)
                 where.append(np.arange(i * width + first, i * width + last + 1, dtype=np.int32))
             where = np.concatenate(where)

@@ -765,7 +765,7 @@ class ReferenceOps:
         starts = retention_start(retention, positions)
         for i in range(n):
             p = int(positions[i])
-            s = int(starts[i])
+            s = max(int(starts[i]), 0)  # (a row at position -1 sees no keys)
             kpos = torch.arange(s, p + 1, device=q.device)
             if keep and s > 0:
                 kpos = torch.cat([torch.arange(0, min(keep, s), device=q.device), kpos])

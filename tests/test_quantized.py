@@ -909,3 +909,58 @@ def test_attention_beside_segments_of_no_tokens(ops, monkeypatch, long):
     c.meta = GroupContext(block_table=c.table, slot_mapping=c.slots, width=c.meta.width, retention=c.rule, seg_lens=[0, 300, 0, 1, 0],
                           seg_starts=[5, 800, 0, 69, 3])
     c.check(c.run(ops))
+
+
+# ------------------------------------------------------------------------------------------------ rows at no position
+@pytest.mark.parametrize("starts", [[-1], [-1, 40], [-1, -1, 700]], ids=str)
+@pytest.mark.parametrize("rule", [("all",), ("chunk", 64), ("window", 100)], ids=str)
+@pytest.mark.timeout(60)
+def test_plans_with_rows_at_no_position(starts, rule):
+    plan = _planner()._quantized_plan([1] * len(starts), starts, rule, 2, 2, 128, 16, None, torch.zeros(len(starts), 50, dtype=torch.int32))
+    (_, num, cols, ranges, keys, _), = plan["few"]
+    assert num == len(starts) and cols == 2 and ranges >= 1 and plan["long"] is None
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param(DEV, marks=gpu)])
+@pytest.mark.parametrize("rule", [("all",), ("chunk", 24), ("window", 19)], ids=str)
+@pytest.mark.parametrize("how", ["single", "lengths", "direct"])
+@pytest.mark.parametrize("ps", [16, 48])
+def test_rows_at_no_position_have_zeros(device, rule, how, ps):
+    """A batch filled up with rows at position -1, of no segment and without a page: zeros, whether the step is laid out for a
+    bound, for its lengths or from its arrays, and the other rows as they are without them."""
+    if device == "cpu":
+        ops = ReferenceOps()
+    else:
+        from jax_llm_examples_amd.engine import get_ops
+        ops = get_ops(device)
+    c = Case([(1, 1), (1, 700), (1, 40), (1, 333)], 4, 2, 64, ps, rule, seed=61, device=device)
+    at = torch.tensor([0, 2, 3, 6], device=device)  # where the rows are among eight
+    q = torch.randn(8, 4, 64, generator=_gen(1)).bfloat16().to(device)
+    q[at] = c.q.to(device)
+    positions, segment = (torch.full((8,), -1, dtype=torch.int32, device=device) for _ in range(2))
+    table = torch.full((8, c.table.shape[1]), -1, dtype=torch.int32, device=device)
+    positions[at], segment[at], table[at] = c.positions, at.to(torch.int32), c.table
+    meta = None if how == "direct" else GroupContext(
+        block_table=table, slot_mapping=positions, width=table.shape[1], retention=rule, seg_lens=[1] * 8,
+        seg_starts=None if how == "single" else positions.tolist(), decode_bucket=1024 if how == "single" else None)
+    if how == "direct":  # (the arrays alone: rows beside each other of one segment are told apart by its number)
+        segment[1], segment[4], segment[5], segment[7] = 1, 4, 5, 7
+    got = ops.paged_attention(q, c.kv, table, positions, segment, rule, c.scale, meta)
+    c.check(got[at])
+    none = torch.ones(8, dtype=torch.bool)
+    none[at.cpu()] = False
+    assert not got.cpu()[none].any()
+
+
+@gpu
+@pytest.mark.parametrize("rule", [("all",), ("chunk", 24), ("window", 19)], ids=str)
+def test_tokens_in_front_of_the_first_position(ops, rule):
+    """Segments of a few tokens of which the first lie in front of position 0: these have zeros, the others their results."""
+    c = Case([(5, 5), (3, 40)], 4, 2, 64, 16, rule, seed=62)
+    c.positions[:5] -= 2
+    c.meta.seg_starts = [-2, 37]
+    got = c.run(ops)
+    assert not got[:2].any()
+    c.cpu = (c.cpu[0], [0, 1, 2, 37, 38, 39], [0, 0, 0, 1, 1, 1])
+    want, tol = c.want(c.q[2:])
+    assert ((got[2:].cpu().double() - want).abs() <= tol).all()
