@@ -129,18 +129,20 @@ def tokens_held_at_most(retention: tuple, max_step_tokens: int, max_seq_len: Opt
 
 def pool_sizes(needs: dict[int, CacheNeed], *, page_size: int, itemsize: int, max_requests: int,
                max_step_tokens: int, max_seq_len: Optional[int] = None, cache_tokens: Optional[int] = None,
-               memory_bytes: Optional[int] = None) -> dict[int, int]:
+               memory_bytes: Optional[int] = None, read_back_bytes: int = 0) -> dict[int, int]:
     """Pages for every group's pool.  Either ``cache_tokens`` (the tokens that a group which keeps
     everything can hold) or ``memory_bytes`` (what all pools together may take: then the largest
     such number of tokens that fits).  A group that lets go of old tokens gets at most what
     ``max_requests`` requests can hold of it (whole pages, and one more per request for a portion
-    that does not start at a page's edge)."""
+    that does not start at a page's edge).  ``read_back_bytes``: what a step's attention over keys and values in 8 bits may
+    hold of them in the run dtype, of one run at a time; ``memory_bytes`` has room for that too, as far as there are pages."""
     groups = plan_groups(needs)
-    caps, page_bytes = [], []
+    caps, page_bytes, read_bytes = [], [], []
     for (kv, paged, retention), cids in groups:
         held = tokens_held_at_most(retention, max_step_tokens, max_seq_len)
         caps.append(None if held is None else max_requests * (-(-held // page_size) + 1))
         page_bytes.append(len(cids) * row_bytes(kv, paged, itemsize) * page_size)
+        read_bytes.append(0 if kv[2] is None else row_bytes((*kv[:2], None), (), itemsize) * page_size)
 
     def sizes(pages_unbounded: int) -> list[int]:
         return [pages_unbounded if c is None else min(c, pages_unbounded) for c in caps]
@@ -149,7 +151,9 @@ def pool_sizes(needs: dict[int, CacheNeed], *, page_size: int, itemsize: int, ma
         want = -(-cache_tokens // page_size)
     elif memory_bytes is not None:
         def total(p):
-            return sum(b * n for b, n in zip(page_bytes, sizes(p)))
+            n = sizes(p)
+            return (sum(b * k for b, k in zip(page_bytes, n))
+                    + min(read_back_bytes, max((b * k for b, k in zip(read_bytes, n)), default=0)))
 
         lo, hi = 0, 1
         while total(hi) <= memory_bytes and hi < (1 << 40):

@@ -334,6 +334,7 @@ __global__ __launch_bounds__(TB > 1 ? TB * 64 * TW : 256, 4) void quantized_prep
 // exact).  Page i is page_ids[where[i]] (where null: page_ids[i]); an id that is no page's gives NaN.  An item is 16 bytes of
 // the result: eight elements of a key, or eight keys of an element of the values; blockIdx: (page, part of its items, keys or
 // values), and a page's items follow each other in the result's order, so that every store of a wavefront is one kilobyte.
+// codes, scales, page_heads: of the first of the Hkv heads that are read, in pages of page_heads.
 // attend: for attention, whose tiles share the values of keys that some of their queries do not see (zero times NaN is NaN): a
 // row of values that is NaN is read as zero, and its key as NaN, which a mask takes away from the queries that do not see it.
 // Memory bounds it: 32,768 tokens of 8 x 128 31 us, 6.5 TB/s, with stores that the caches need not keep (with others 37 to 46).
@@ -345,15 +346,15 @@ __device__ __forceinline__ uint32_t two_bf16(uint32_t w, float scale, bool hi) {
 __global__ __launch_bounds__(256) void quantized_read_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                              const int* __restrict__ page_ids,
                                                              const int* __restrict__ where, bf16_t* __restrict__ out,
-                                                             int num_pages, int attend, int Hkv, int ps, int dh, Divisor plane_items,
+                                                             int num_pages, int attend, int page_heads, int Hkv, int ps, int dh, Divisor plane_items,
                                                              Divisor row_keys, Divisor row_values) {
   const int i = blockIdx.x, which = blockIdx.z;
   const int page = page_ids[where != nullptr ? where[i] : i];
   const bool ok = page >= 0 && page < num_pages;
   const int items = Hkv * (int)plane_items.d;
   const size_t plane_codes = (size_t)ps * dh;
-  const uint8_t* cp = codes + ((size_t)(ok ? page : 0) * Hkv * 2 + which) * plane_codes;  // head h: + 2 h planes
-  const uint8_t* sp = scales + ((size_t)(ok ? page : 0) * Hkv * 2 + which) * ps;
+  const uint8_t* cp = codes + ((size_t)(ok ? page : 0) * page_heads * 2 + which) * plane_codes;  // head h: + 2 h planes
+  const uint8_t* sp = scales + ((size_t)(ok ? page : 0) * page_heads * 2 + which) * ps;
   bf16_t* dst = out + ((size_t)i * 2 + which) * Hkv * plane_codes;
   const int first = blockIdx.y * (256 * kReadItems) + threadIdx.x;
   u32x2 c[kReadItems], f[kReadItems];
@@ -459,15 +460,18 @@ JLE_API int jle_quantized_prepare(const void* qkv, void* q_out, void* codes, voi
 }
 
 JLE_API int jle_quantized_read(const void* codes, const void* scales, const int* page_ids, const int* where, void* out,
-                               int n, int num_pages, int attend, int Hkv, int dh, int ps, hipStream_t s) {
+                               int n, int num_pages, int attend, int page_heads, int first_head, int Hkv, int dh, int ps,
+                               hipStream_t s) {
   if (n <= 0) return 0;
   if (!jle_quantized_supported(dh, Hkv, Hkv, ps) || num_pages <= 0) return JLE_BAD_ARG;
+  if (first_head < 0 || first_head > page_heads - Hkv) return JLE_BAD_ARG;
   if (((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)out) & 15) return JLE_BAD_ARG;
   const long long items = (long long)Hkv * ps * (dh / 8);
   const long long parts = (items + 256 * kReadItems - 1) / (256 * kReadItems);
   if (parts > 65535) return JLE_BAD_ARG;
-  hipLaunchKernelGGL(quantized_read_kernel, dim3(n, (unsigned)parts, 2), dim3(256), 0, s, (const uint8_t*)codes,
-                     (const uint8_t*)scales, page_ids, where, (bf16_t*)out, num_pages, attend, Hkv, ps, dh, divisor(ps * (dh / 8)),
+  hipLaunchKernelGGL(quantized_read_kernel, dim3(n, (unsigned)parts, 2), dim3(256), 0, s,
+                     (const uint8_t*)codes + (size_t)first_head * 2 * ps * dh, (const uint8_t*)scales + (size_t)first_head * 2 * ps,
+                     page_ids, where, (bf16_t*)out, num_pages, attend, page_heads, Hkv, ps, dh, divisor(ps * (dh / 8)),
                      divisor(dh / 8), divisor(ps / 8));
   JLE_LAUNCH_CHECK();
   return 0;

@@ -37,7 +37,8 @@ class Engine:
         hold of them.  ``max_seq_len``: a request ends with reason ``"length"`` when prompt and
         output reach it; default: the configuration's ``max_position_embeddings``, if it has one.
         ``kv_dtype``: ``"float8_e4m3"`` holds the attention layers' keys and values in 8 bits, each row with a power of two
-        of its own (about half the bytes of bfloat16; ``ValueError`` where a layer cannot have it so).
+        of its own (about half the bytes of bfloat16; ``ValueError`` where a layer cannot have it so); where the pools are
+        sized by memory, what a portion's attention reads back at once (at most 2 GiB) is taken off first.
         ``decode_graphs``: replay steps of single tokens as recorded HIP graphs (default: on a GPU)."""
         self.model = model
         self.max_num_batched_tokens = max_num_batched_tokens
@@ -73,7 +74,8 @@ class Engine:
                 raise ValueError("give cache_tokens, kv_memory_fraction or max_seq_len")
         num_pages = pool_sizes(needs, page_size=page_size, itemsize=item, max_requests=decode_batch_size,
                                max_step_tokens=max_num_batched_tokens, max_seq_len=max_seq_len,
-                               cache_tokens=cache_tokens, memory_bytes=memory)
+                               cache_tokens=cache_tokens, memory_bytes=memory,
+                               read_back_bytes=getattr(self.ops, "QUANTIZED_READ_BYTES", 0))
         self.cache = CacheManager(needs, page_size=page_size, num_pages=num_pages,
                                   max_requests=decode_batch_size, dtype=model.dtype, device=model.device,
                                   poison=poison, run_states=model.run_state_needs())

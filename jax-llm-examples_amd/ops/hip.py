@@ -134,7 +134,7 @@ _SIGNATURES = {
                                  _vp, _vp],
     "jle_quantized_prepare": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _vp, _vp, _i, _i, _f, _f, _i, _i, _i, _i, _i, _i, _vp,
                               _i, _vp],
-    "jle_quantized_read": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
+    "jle_quantized_read": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
     "jle_attention_quantized": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _i,
                                 _i, _i, _vp],
     "jle_paged_attention_biased": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _i, _i, _i, _i, _i, _i, _i, _i, _vp,
@@ -2645,8 +2645,8 @@ class HipOps:
         self._here(page_ids, "page ids", 4)
         return self._read_pages(kv, page_ids, None)
 
-    def _read_pages(self, kv, page_ids, where):
-        """``where``: the places of ``page_ids`` that are meant, for the attention kernels over bfloat16, whose tiles share the
+    def _read_pages(self, kv, page_ids, where, heads=None):
+        """``heads``: the first of the kv heads that are meant and the one behind the last (None: all).  ``where``: the places of ``page_ids`` that are meant, for the attention kernels over bfloat16, whose tiles share the
         values: a row of values that is NaN is then zeros and its key NaN, which the mask keeps from queries that do not see it
         (None: all pages, one after the other, as they are)."""
         p, _, hk, ps, dh = kv.shape
@@ -2655,12 +2655,21 @@ class HipOps:
         if p == 0:
             raise KernelError("no pages to read")
         n = page_ids.numel() if where is None else where.numel()
-        out = torch.empty(n, 2, hk, ps, dh, dtype=torch.bfloat16, device=kv.device)
+        first, end = heads or (0, hk)
+        size = n * 2 * (end - first) * ps * dh
+        # (for attention a power of two: a prompt's portions, each with more pages than the last, ask for few different sizes, and
+        # the allocator has what the last one gave back)
+        out = torch.empty(size if where is None else 1 << (size - 1).bit_length(), dtype=torch.bfloat16, device=kv.device)
+        out = out[:size].view(n, 2, end - first, ps, dh)
         self._call("jle_quantized_read", kv.codes.data_ptr(), kv.scales.data_ptr(), page_ids.data_ptr(), _p(where), out.data_ptr(),
-                   n, p, int(where is not None), hk, dh, ps)
+                   n, p, int(where is not None), hk, first, end - first, dh, ps)
         return out
 
-    QUANTIZED_TOKENS = 4096  # a segment of more tokens never takes the kernel over codes
+    QUANTIZED_TOKENS = 4096  # a segment of more tokens takes the kernel over codes only where its pages are too many to read back
+    # Pages read back at once, in bytes of bfloat16 (a power of two): 524,288 keys of 8 kv heads of 128.  The longer contexts are
+    # read back in runs of kv heads (2,048 tokens of 40 heads on 300,000 keys 16.2 ms in one, 20.1 in three), and go through the
+    # codes (52 ms) where one head's keys are more, beyond 4,194,304 of 128.
+    QUANTIZED_READ_BYTES = 1 << 31
     QUANTIZED_RANGES = 64  # of a (tile, kv head), at most
     # Measured on MI355X, bfloat16 queries.  The kernel over codes: a block of eight wavefronts with up to 16 columns works
     # through a key in 4.8 ns at head size 128 (98 to 32,768 keys), 1.8, 2.8, 3.8 and 9 at 32, 64, 96 and 256; with up to 32
@@ -2710,10 +2719,12 @@ class HipOps:
 
     def _quantized_plan(self, seg_lens, seg_starts, retention, num_kv_heads: int, group: int, head_dim: int, page_size: int,
                         decode_bucket, block_table):
-        """What a step's attention over pages in 8 bits is made of.  ``few``: for single tokens and for segments of not so many
-        tokens that this kernel is the slower one, their tiles (as many tokens as 16 columns hold, or one), the columns, the
-        ranges; ``long``: for the others, the tiles of the attention kernel over pages in bfloat16, the pages that it needs
-        read back and the block table over those."""
+        """What a step's attention over pages in 8 bits is made of.  ``few``: for single tokens, for segments of not so many
+        tokens that this kernel is the slower one and for those of which not one head's pages may be read back at once
+        (``QUANTIZED_READ_BYTES``), their tiles (as many tokens as 16 columns hold, or one), the columns, the ranges; ``long``:
+        for the others, in passes whose pages are no more than that, the tiles of the attention kernel over pages in bfloat16,
+        the pages that it needs read back, the block table over those and, where all kv heads of a segment are too many, its
+        rows and which heads (the first, and the one behind the last, of both)."""
         from ..parts.base import first_needed_position
 
         device = block_table.device
@@ -2754,6 +2765,16 @@ class HipOps:
 
         plan = {"few": [], "long": None, "tokens": int(offsets[-1])}
         long = []
+        ps, width = page_size, block_table.shape[1]
+
+        def pages_of(i):
+            """The places in its row of the block table that segment ``i`` reads: the first, and the one behind the last."""
+            first = first_needed_position(retention, max(seg_starts[i], 0)) // ps
+            return first, max(first, min((seg_starts[i] + seg_lens[i] - 1) // ps, width - 1) + 1)
+
+        def read_bytes(i):
+            first, end = pages_of(i)
+            return (end - first) * num_kv_heads * ps * head_dim * 4
         if decode_bucket is not None:  # (single tokens; the same for all steps of so many requests below this bound)
             n = len(seg_lens)
             held = decode_bucket if retention[0] == "all" else min(decode_bucket, int(retention[1]))
@@ -2766,14 +2787,14 @@ class HipOps:
             plan["few"].append((None, n, group, *split[1:], {}))
         else:
             # segments of up to so many tokens go through the kernel over codes: the bound with which the step is done first
-            short = [i for i, n in enumerate(seg_lens) if 0 < n <= tokens]
+            heavy = {i for i, n in enumerate(seg_lens) if n > tokens and read_bytes(i) // num_kv_heads > self.QUANTIZED_READ_BYTES}
+            few = lambda bound: [i for i, n in enumerate(seg_lens) if 0 < n <= bound or i in heavy]
             lengths = sorted({n for n in seg_lens if tokens < n <= self.QUANTIZED_TOKENS})
             if len(lengths) > 6:
                 lengths = lengths[:: -(-len(lengths) // 6)] + lengths[-1:]
             best = None
             for bound in [tokens, *lengths]:
-                mine = short if bound == tokens else [i for i, n in enumerate(seg_lens) if 0 < n <= bound]
-                rest = [i for i, n in enumerate(seg_lens) if n > bound]
+                mine, rest = few(bound), [i for i, n in enumerate(seg_lens) if n > bound and i not in heavy]
                 tiles, split = few_of(mine) if mine else (None, (0.0,))
                 cost = split[0] + long_us(rest)
                 if best is None or cost < best[0]:
@@ -2785,21 +2806,29 @@ class HipOps:
                     listed = to_device(torch.from_numpy(tiles.astype(np.int32)), device)
                 plan["few"].append((listed, len(tiles), int(tiles[:, 1].max()) * group, *split[1:], {}))
         plan["tickets"] = sum(num * num_kv_heads for _, num, _, ranges, _, _ in plan["few"] if ranges > 1)
-        if long:
-            ps, width = page_size, block_table.shape[1]
-            where = []
-            for i in long:
-                first = first_needed_position(retention, max(seg_starts[i], 0)) // ps
-                last = min((seg_starts[i] + seg_lens[i] - 1) // ps, width - 1)
-                where.append(np.arange(i * width + first, i * width + last + 1, dtype=np.int32))
-            where = np.concatenate(where)
+        passes, held = [], self.QUANTIZED_READ_BYTES
+        for i in long:
+            held += read_bytes(i)
+            if held > self.QUANTIZED_READ_BYTES:
+                passes.append([])
+                held = read_bytes(i)
+            passes[-1].append(i)
+        for segments in passes:
+            where = np.concatenate([np.arange(i * width + first, i * width + end, dtype=np.int32)
+                                    for i in segments for first, end in (pages_of(i),)])
             table = np.full(block_table.numel(), -1, np.int32)
             table[where] = np.arange(where.size, dtype=np.int32)
             sent = to_device(torch.from_numpy(np.concatenate([where, table])), device)
             where, table = sent[: where.size], sent[where.size:].view(block_table.shape)
             tiles = self.attention_plan(seg_lens, seg_starts, retention, device, num_kv_heads, group, single_tiles=True,
-                                        only=set(long))
-            plan["long"] = (tiles, where, table)
+                                        only=set(segments))
+            heads, parts = num_kv_heads, (None,)
+            if sum(map(read_bytes, segments)) > self.QUANTIZED_READ_BYTES:  # (one segment; as many heads as may be, about alike)
+                i, = segments
+                heads = self.QUANTIZED_READ_BYTES // (read_bytes(i) // num_kv_heads)
+                heads = -(-num_kv_heads // -(-num_kv_heads // heads))
+                parts = [(int(offsets[i]), int(offsets[i + 1]), h, min(h + heads, num_kv_heads)) for h in range(0, num_kv_heads, heads)]
+            plan["long"] = [*(plan["long"] or ()), *((tiles, where, table, part) for part in parts)]
         return plan
 
     def _quantized_plan_of(self, meta, token_segment, positions, retention, hq: int, kv, block_table):
@@ -2868,12 +2897,21 @@ class HipOps:
                        ws_o, mine, positions.data_ptr(), token_segment.data_ptr(), block_table.data_ptr(), block_table.shape[1],
                        p, None if tiles is None else tiles.data_ptr(), num, cols, ranges, span, mode, param, float(scale), hq,
                        hk, dh, ps)
-        if plan["long"] is not None:
-            tiles, where, table = plan["long"]
-            pages = self._read_pages(kv, block_table, where)
-            self._call("jle_attention_prefill", _p(q), _p(pages), _p(out), _p(positions), _p(token_segment), _p(table),
+        for tiles, where, table, part in plan["long"] or ():
+            first, end = (0, hk) if part is None else part[2:]
+            pages = self._read_pages(kv, block_table, where, (first, end))
+            mine, q_mine = out, q
+            if part is not None:  # (these heads' queries, as the kernel reads them)
+                q_mine = q.view(n, hk, -1)[:, first:end].contiguous()
+                mine = torch.empty_like(q_mine)
+            self._call("jle_attention_prefill", _p(q_mine), _p(pages), _p(mine), _p(positions), _p(token_segment), _p(table),
                        table.shape[1], _p(tiles["tiles"]), tiles["num_tiles"], self.PREFILL_TILE, _p(tiles["groups"]),
-                       tiles["num_groups"], mode, param, float(scale), hq, hk, dh, ps, None, 0, None, 0.0)
+                       tiles["num_groups"], mode, param, float(scale), (end - first) * (hq // hk), end - first, dh, ps, None, 0,
+                       None, 0.0)
+            if part is not None:
+                rows = slice(part[0], part[1])
+                out.view(n, hk, -1)[rows, first:end] = mine[rows]
+            del pages  # (the next pass has the same memory)
         return out
 
     # ------------------------------------------------------------------ routed experts

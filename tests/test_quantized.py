@@ -964,3 +964,131 @@ def test_tokens_in_front_of_the_first_position(ops, rule):
     c.cpu = (c.cpu[0], [0, 1, 2, 37, 38, 39], [0, 0, 0, 1, 1, 1])
     want, tol = c.want(c.q[2:])
     assert ((got[2:].cpu().double() - want).abs() <= tol).all()
+
+
+# ------------------------------------------------------------------------------------------------ pages read back at once
+LONG = [(300, 2000), (1, 70), (600, 600), (40, 9000), (5000, 5000), (33, 8000), (3, 20_000), (64, 700)]
+
+
+@pytest.mark.parametrize("limit", [1 << 19, 1 << 21, 1 << 22, 1 << 24])
+@pytest.mark.parametrize("rule", [("all",), ("chunk", 1024), ("window", 3000)], ids=str)
+@pytest.mark.parametrize("codes", [0, 4096])
+def test_plans_read_back_no_more_than_the_bound_at_once(limit, rule, codes):
+    """What goes the long way is read back in passes of no more than the bound, several segments at once or some of a segment's
+    heads; a segment of which one head's pages are more than that goes through the codes, whatever its length; every token and
+    head is in one place."""
+    ops = _planner()
+    ops.QUANTIZED_READ_BYTES, ops.QUANTIZED_TOKENS = limit, codes
+    hk, dh, ps = 3, 64, 16
+    lens, starts = [n for n, _ in LONG], [t - n for n, t in LONG]
+    table = torch.zeros(len(LONG), -(-20_000 // ps), dtype=torch.int32)
+    plan = ops._quantized_plan(lens, starts, rule, hk, 4, dh, ps, None, table)
+    done = torch.zeros(sum(lens), hk, dtype=torch.int32)
+    for tiles, num, *_ in plan["few"]:
+        for first, n in (tiles.tolist() if tiles is not None else [(i, 1) for i in range(num)]):
+            done[first: first + n] += 1
+    first_row = [sum(lens[:i]) for i in range(len(lens))]
+    of = {i: Case.first(type("R", (), {"rule": rule})(), s) // ps for i, s in enumerate(starts)}
+    head = {i: ((starts[i] + lens[i] - 1) // ps + 1 - of[i]) * ps * dh * 4 for i in of}
+    for tiles, where, mapped, part in plan["long"] or ():
+        low, high = (0, hk) if part is None else part[2:]
+        assert 0 < where.numel() * (high - low) * ps * dh * 4 <= limit
+        assert torch.equal(mapped.view(-1)[where.long()], torch.arange(where.numel(), dtype=torch.int32)) and int((mapped >= 0).sum()) == where.numel()
+        for first, n in tiles["tiles"].view(-1, 2).tolist():
+            done[first: first + n, low:high] += 1
+            i = max(j for j in of if first_row[j] <= first)
+            assert (mapped[i, of[i]: (starts[i] + lens[i] - 1) // ps + 1] >= 0).all()
+            assert part is None or part[:2] == (first_row[i], first_row[i] + lens[i])
+    assert (done == 1).all()
+    if codes == 0:  # (only what is too much takes the codes, and single tokens and tiles of a few)
+        few = {max(j for j in of if first_row[j] <= first) for first, _ in plan["few"][0][0].tolist()}
+        assert few == {i for i in of if lens[i] <= 4 or head[i] > limit}
+
+
+@gpu
+@pytest.mark.parametrize("rule", [("all",), ("chunk", 256), ("window", 300)], ids=str)
+@pytest.mark.parametrize("limit", [1 << 18, 1 << 19, 1 << 20])
+@pytest.mark.parametrize("hq,hk,dh", [(10, 2, 128), (6, 3, 128), (8, 4, 32)])
+def test_pages_read_back_in_passes(ops, monkeypatch, rule, limit, hq, hk, dh):
+    """A bound that only some of the segments keep, one by one, and some in runs of heads: results as ever, bit for bit where
+    the segments' tiles are the same, and no more memory than the bound at once (beside a run's queries and results)."""
+    monkeypatch.setattr(type(ops), "QUANTIZED_TOKENS", 0)
+    c = Case([(70, 70), (1, 300), (33, 215), (5, 12), (129, 400), (40, 2300), (17, 1000), (64, 64)], hq, hk, dh, 16, rule, seed=71)
+    at_once = c.run(ops)
+    c.check(at_once)
+    monkeypatch.setattr(type(ops), "QUANTIZED_READ_BYTES", limit)
+    c.meta.meta.clear()
+    q = c.q.to(DEV)
+    c.check(c.run(ops, q))  # (its plan)
+    plan = next(v for k, v in c.meta.meta.items() if isinstance(k, tuple) and k[0] == "quantized_plan")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = c.run(ops, q)
+    assert torch.cuda.max_memory_allocated() - before <= limit + 3 * got.numel() * 2 + 8192
+    c.check(got)
+    many = [n for n, _ in c.segs]
+    for _, where, table, part in plan["long"]:
+        assert where.numel() * dh * 16 * 4 * (hk if part is None else part[3] - part[2]) <= limit
+        for i in range(len(many)):
+            if (table[i] >= 0).any():
+                rows = slice(sum(many[:i]), sum(many[: i + 1]))
+                assert torch.equal(got[rows], at_once[rows])
+
+
+@gpu
+def test_portions_of_a_growing_context_ask_for_few_sizes(ops):
+    """Each portion reads back more pages than the one before: the allocator's memory grows by no more than twice the last's."""
+    hq, hk, dh, ps, n, width = 8, 8, 128, 16, 600, 3000
+    kv = QuantizedPages.empty(width, hk, ps, dh, DEV)
+    table = torch.arange(width, dtype=torch.int32, device=DEV).view(1, -1)
+    q = torch.randn(n, hq, dh, generator=_gen(1)).bfloat16().to(DEV)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    before = torch.cuda.memory_reserved()
+    for start in range(0, width * ps - n, n):
+        positions = torch.arange(start, start + n, dtype=torch.int32, device=DEV)
+        meta = GroupContext(block_table=table, slot_mapping=positions, width=width, retention=("all",), seg_lens=[n], seg_starts=[start])
+        with pytest.MonkeyPatch.context() as m:
+            m.setattr(type(ops), "QUANTIZED_TOKENS", 0)
+            ops.paged_attention(q, kv, table, positions, torch.zeros_like(positions), ("all",), 0.1, meta)
+    last = width * ps * hk * dh * 4
+    assert torch.cuda.memory_reserved() - before <= 4 * last + (64 << 20)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+
+
+def test_pool_sizes_by_memory_leave_room_for_what_is_read_back(model_dirs_bf16):
+    """As many pages as the memory holds beside one run's pages in bfloat16, or beside the bound where that is less."""
+    from jax_llm_examples_amd import load_model
+    from jax_llm_examples_amd.cache import plan_groups, pool_sizes
+    from jax_llm_examples_amd.cache.manager import row_bytes
+
+    model = load_model(model_dirs_bf16["B"], "bfloat16", "cpu")
+    for kv_dtype in (None, "float8_e4m3"):
+        needs = model.cache_needs(kv_dtype)
+        groups = plan_groups(needs)
+        kw = dict(page_size=16, itemsize=2, max_requests=4, max_step_tokens=64)
+        for memory in (1 << 20, 1 << 22):
+            for bound in (0, 1 << 16, 1 << 30):
+                def taken(n):
+                    pools = sum(n[i] * 16 * len(cids) * row_bytes(kv, paged, 2) for i, ((kv, paged, _), cids) in enumerate(groups))
+                    most = max(n[i] * 16 * 2 * kv[0] * kv[1] * 2 for i, ((kv, _, _), _) in enumerate(groups))
+                    return pools + (min(bound, most) if kv_dtype else 0)
+                n = pool_sizes(needs, memory_bytes=memory, read_back_bytes=bound, **kw)
+                assert taken(n) <= memory < taken({i: k + 1 for i, k in n.items()})
+                if kv_dtype is None:
+                    assert n == pool_sizes(needs, memory_bytes=memory, **kw)
+
+
+def test_engine_sizes_its_pools_with_room_for_what_is_read_back(model_dirs_bf16, monkeypatch):
+    from jax_llm_examples_amd.engine import engine as module
+
+    seen = []
+    real = module.pool_sizes
+    monkeypatch.setattr(module, "pool_sizes", lambda needs, **kw: seen.append(kw) or real(needs, **kw))
+    monkeypatch.setattr(ReferenceOps, "QUANTIZED_READ_BYTES", 12_345, raising=False)
+    _engine(model_dirs_bf16["B"], "cpu")
+    assert seen[0]["read_back_bytes"] == 12_345
+    from jax_llm_examples_amd.ops.hip import HipOps
+    assert HipOps.QUANTIZED_READ_BYTES == 1 << 31
