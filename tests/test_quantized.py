@@ -1092,3 +1092,59 @@ def test_engine_sizes_its_pools_with_room_for_what_is_read_back(model_dirs_bf16,
     assert seen[0]["read_back_bytes"] == 12_345
     from jax_llm_examples_amd.ops.hip import HipOps
     assert HipOps.QUANTIZED_READ_BYTES == 1 << 31
+
+
+# ------------------------------------------------------------------------------------------------ rows of portions
+def _check_written(ops, n, hq, hk, dh, ps, kind, seed, pos):
+    """Rows in places that begin nowhere in particular, jump, run backwards and leave some out: every value's code and scale, a
+    key's code but where its 64-bit number lies within 2^-44 of the row's longest of a border, queries, and nothing else."""
+    g = _gen(seed)
+    qkv = (torch.randn(n, hq + 2 * hk, dh, generator=g) * torch.exp2(torch.randint(-6, 7, (n, hq + 2 * hk, 1), generator=g).float())).bfloat16()
+    qkv[0, hq + hk] = 0.0  # a value of zeros
+    qkv[n // 2, hq + 2 * hk - 1, 3] = float("inf")  # one that is held as NaN
+    P = (n + 3) // ps + 3
+    order = torch.randperm(P, generator=g)
+    slots = torch.tensor([int(order[i // ps]) * ps + i % ps for i in range(3, 3 + n)], dtype=torch.int32)
+    slots[17:41] = slots[17:41].flip(0)  # (backwards)
+    slots[60:70] = slots[60:70][torch.randperm(10, generator=g)]
+    slots[2], slots[4], slots[9], slots[46], slots[90], slots[n - 1] = -1, P * ps, -5, -1, 2 ** 31 - 1, -1
+    kv = QuantizedPages.empty(P, hk, ps, dh, DEV, poison=True)
+    q = ops.qk_prepare_kv_write(qkv.view(n, -1).to(DEV), hq, hk, dh, torch.tensor(pos, dtype=torch.int32, device=DEV), _prep(kind, dh, DEV),
+                                kv, slots.to(DEV)).cpu().double()
+    wq, wk, wv = _prepared(qkv.view(n, -1), hq, hk, dh, pos, _prep(kind, dh))
+    # (as in the test of a few rows: 64 roundings of float32 of the longest number, and bfloat16's)
+    assert ((q - wq).abs() <= 2.0 ** -8 * wq.abs() + 64 * 2.0 ** -24 * (wq.abs() + wq.abs().amax(-1, keepdim=True))).all()
+    codes, scales = kv.codes.cpu(), kv.scales.cpu()
+    there = ((slots >= 0) & (slots < P * ps)).nonzero().view(-1)
+    s = slots[there].long()
+    assert s.unique().numel() == s.numel()
+    k, v = (x.double().transpose(1, 2)[s // ps, s % ps] for x in Q.read_rows(QuantizedPages(codes, scales), torch.arange(P)))
+    want, e = held(wv[there])
+    bad = ~torch.isfinite(wv[there]).all(-1)
+    assert bad.any() and v[bad].isnan().all() and torch.equal(v[~bad], want[~bad])
+    assert torch.equal(scales[s // ps, :, 1, s % ps].double()[~bad] - 127, e[~bad])
+    slack = 2.0 ** -44 * wk[there].abs().amax(-1, keepdim=True)
+    low, high = held(wk[there] - slack)[0], held(wk[there] + slack)[0]
+    assert ((k == low) | (k == high)).all()
+    untouched = torch.ones(P * ps, dtype=torch.bool)
+    untouched[s] = False
+    assert (scales.permute(0, 3, 1, 2).reshape(P * ps, -1)[untouched] == Q.NAN_CODE).all()
+    for x in Q.read_rows(QuantizedPages(codes, torch.full_like(scales, 127)), torch.arange(P)):
+        assert x.transpose(1, 2).reshape(P * ps, -1)[untouched].isnan().all()
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["none", "plain", "half", "half part", "first", "weighted"])
+@pytest.mark.parametrize("hq,hk,dh", [(3, 1, 32), (4, 2, 64), (3, 3, 96), (10, 2, 128), (2, 1, 256), (16, 16, 128), (8, 8, 256)])
+def test_portions_are_written_row_by_row(ops, kind, hq, hk, dh):
+    """From 127 tokens, one a block, on 128, where a block takes eight (the last two: heads that do not fit there)."""
+    for n, ps in ((127, 16), (128, 48), (131, 16), (200, 16)):
+        _check_written(ops, n, hq, hk, dh, ps, kind, n + dh, list(range(5, 5 + n)))
+
+
+@gpu
+@pytest.mark.parametrize("kind,hq,hk,dh", [("plain", 3, 1, 32), ("half part", 4, 2, 64), ("first", 3, 3, 96), ("none", 4, 2, 128), ("weighted", 2, 1, 256)])
+def test_portions_of_thousands_are_written_row_by_row(ops, kind, hq, hk, dh):
+    """On both sides of the number of tokens from which a wavefront takes one by itself."""
+    for n in (4096, 4097, 5003):
+        _check_written(ops, n, hq, hk, dh, 16, kind, n, [(7919 * i) % 1_000_003 for i in range(n)])
