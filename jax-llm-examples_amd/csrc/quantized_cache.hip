@@ -144,8 +144,9 @@ __device__ __forceinline__ void prepare_head(F (&x)[8], const PrepareArgs& a, co
 // With one token a block (few tokens) the units are shared out among gridDim.y blocks of four wavefronts and the codes go
 // straight into their pages (one token of 56 heads 4.3 us, 64 of 32 5.2); with several TW wavefronts share a token, the codes
 // are gathered in shared memory and written in larger pieces (8,191 tokens of 48 heads of 128: 48 us, 3.9 TB/s, 98 when every
-// value was stored by itself; vector instructions bound it, 1,850 a token and wavefront): keys eight codes each, the tokens' side by side, values the four keys of four elements in 16 bytes where
-// the block's tokens fill an aligned four of a page (other values byte by byte).
+// value was stored by itself; vector instructions bound it, 1,850 a token and wavefront): keys eight codes each, the tokens'
+// side by side, values the four keys of four elements in 16 bytes where the block's tokens fill an aligned four of a page (other
+// values byte by byte).
 template <int LPH, int TB, int TW>
 __global__ __launch_bounds__(TB > 1 ? TB * 64 * TW : 256, 4) void quantized_prepare_kernel(PrepareArgs a) {
   constexpr int HPW = 64 / LPH, THREADS = TB > 1 ? TB * 64 * TW : 256;
@@ -330,8 +331,8 @@ __global__ __launch_bounds__(TB > 1 ? TB * 64 * TW : 256, 4) void quantized_prep
   }
 }
 
-// Pages in bfloat16, in the layout of the attention kernels (keys [page_size][dh], values [dh][page_size]; every number is
-// exact).  Page i is page_ids[where[i]] (where null: page_ids[i]); an id that is no page's gives NaN.  An item is 16 bytes of
+// Pages in bfloat16, in the layout of the attention kernels (keys [page_size][dh], values [dh][page_size]; exact wherever
+// bfloat16 holds the number: not below 2^-126, nor a code times its scale of 2^128).  Page i is page_ids[where[i]] (where null: page_ids[i]); an id that is no page's gives NaN.  An item is 16 bytes of
 // the result: eight elements of a key, or eight keys of an element of the values; blockIdx: (page, part of its items, keys or
 // values), and a page's items follow each other in the result's order, so that every store of a wavefront is one kilobyte.
 // codes, scales, page_heads: of the first of the Hkv heads that are read, in pages of page_heads.
@@ -406,7 +407,7 @@ __global__ __launch_bounds__(256) void quantized_read_kernel(const uint8_t* __re
   }
 }
 
-JLE_API int jle_quantized_supported(int dh, int Hq, int Hkv, int ps) {
+static bool sizes_ok(int dh, int Hq, int Hkv, int ps) {
   return quantized_head_ok(dh) && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= 32 && ps >= 16 && ps % 16 == 0;
 }
 
@@ -416,7 +417,7 @@ JLE_API int jle_quantized_prepare(const void* qkv, void* q_out, void* codes, voi
                                   float floor_scale, float attn_scale, int N, int Hq, int Hkv, int dh, int ps,
                                   int num_pages, int* clear, int num_clear, hipStream_t s) {
   if (N <= 0) return 0;
-  if (!jle_quantized_supported(dh, Hq, Hkv, ps) || num_pages < 0) return JLE_BAD_ARG;
+  if (!sizes_ok(dh, Hq, Hkv, ps) || num_pages < 0) return JLE_BAD_ARG;
   if ((codes == nullptr) != (scales == nullptr) || (codes != nullptr && slot_mapping == nullptr)) return JLE_BAD_ARG;
   if (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)codes) & 15) return JLE_BAD_ARG;
   if (num_clear < 0 || (num_clear > 0 && clear == nullptr) || (long long)num_pages * ps > 0x7fffffffll) return JLE_BAD_ARG;
@@ -431,7 +432,9 @@ JLE_API int jle_quantized_prepare(const void* qkv, void* q_out, void* codes, voi
                          clear, num_clear};
   const int hpw = 64 / lph;
   const int units = (Hq + hpw - 1) / hpw + (codes != nullptr ? 2 * ((Hkv + hpw - 1) / hpw) : 0);
-  // Several tokens a block from kManyTokens on, where their codes fit a quarter of the shared memory.
+  // Several tokens a block from kManyTokens on, where their codes fit a quarter of the shared memory: with the whole head turned
+  // up to 14 kv heads of 128, 32 of 64, 4 of 256.  With more, one token a block at any number, whose values are stored code by
+  // code (2,048 tokens of 32 heads of 128 with 8, 16 and 32 kv heads: 24, 44 and 63 us; 8,191 with 8 and 32: 55 and 207).
   const size_t turns = (size_t)pairs * (sizeof(double2) + sizeof(float2));
   const size_t lds = kTokens * (turns + 2 * (size_t)Hkv * dh);
   const bool many = N >= kManyTokens && lds <= 40 * 1024;
@@ -463,7 +466,7 @@ JLE_API int jle_quantized_read(const void* codes, const void* scales, const int*
                                int n, int num_pages, int attend, int page_heads, int first_head, int Hkv, int dh, int ps,
                                hipStream_t s) {
   if (n <= 0) return 0;
-  if (!jle_quantized_supported(dh, Hkv, Hkv, ps) || num_pages <= 0) return JLE_BAD_ARG;
+  if (!sizes_ok(dh, Hkv, Hkv, ps) || num_pages <= 0) return JLE_BAD_ARG;
   if (first_head < 0 || first_head > page_heads - Hkv) return JLE_BAD_ARG;
   if (((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)out) & 15) return JLE_BAD_ARG;
   const long long items = (long long)Hkv * ps * (dh / 8);

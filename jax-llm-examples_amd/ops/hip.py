@@ -2639,8 +2639,8 @@ class HipOps:
 
     def read_pages(self, kv: QuantizedPages, page_ids):
         """The given pages (int32, on the device) of a cache in 8 bits, in bfloat16 and in the layout in which the attention
-        kernels read pages, ``[n, 2, kv_heads, page_size, head_dim]``; every number is exact.  An id that is no page's gives
-        NaN."""
+        kernels read pages, ``[n, 2, kv_heads, page_size, head_dim]``; exact wherever bfloat16 holds the number (magnitudes below
+        2^-126 may be rounded or zero, a code times its scale of 2^128 is infinite).  An id that is no page's gives NaN."""
         self._chk(page_ids, torch.int32, (page_ids.numel(),), "page ids")
         self._here(page_ids, "page ids", 4)
         return self._read_pages(kv, page_ids, None)
