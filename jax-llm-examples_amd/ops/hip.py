@@ -2622,12 +2622,12 @@ class HipOps:
             if not 0 < rd <= dh or rd % (16 if pairing else 2):
                 raise KernelError(f"rotary/norm kernel: {rd} rotated elements of a head of {dh} (half-split pairs: a multiple "
                                   "of 16)")
-            self._chk(inv_freq, torch.float32, (rd // 2,), "inv_freq")
+            self._here(self._chk(inv_freq, torch.float32, (rd // 2,), "inv_freq"), "inv_freq", 4)
         for w, what in ((prep.norm_weight_q, "q norm weight"), (prep.norm_weight_k, "k norm weight")):
             if w is not None:
                 if prep.norm_eps is None:
                     raise KernelError("rotary/norm kernel: norm weights without a norm")
-                self._chk(w, torch.float32, (dh,), what)
+                self._here(self._chk(w, torch.float32, (dh,), what), what, 4)
         q = torch.empty(n, hq, dh, dtype=qkv.dtype, device=qkv.device)
         fs, sc = (prep.query_scale if prep.query_scale is not None else (0.0, 0.0))
         self._call("jle_quantized_prepare", _p(qkv), _p(q), _p(kv.codes) if writes else None,

@@ -1148,3 +1148,26 @@ def test_portions_of_thousands_are_written_row_by_row(ops, kind, hq, hk, dh):
     """On both sides of the number of tokens from which a wavefront takes one by itself."""
     for n in (4096, 4097, 5003):
         _check_written(ops, n, hq, hk, dh, 16, kind, n, [(7919 * i) % 1_000_003 for i in range(n)])
+
+
+# ------------------------------------------------------------------------------------------------ arguments on another device
+@pytest.mark.parametrize("which", ["inv_freq", "q norm weight", "k norm weight"])
+def test_preparation_refuses_what_lies_on_another_gpu(which):
+    """What no launch may read: tensors of a second GPU (by what the checks look at of them)."""
+    import types
+
+    from jax_llm_examples_amd.ops.hip import KernelError
+
+    def tensor(dtype, *shape, device=0):
+        return types.SimpleNamespace(dtype=dtype, shape=torch.Size(shape), device=torch.device("cuda", device), is_cuda=True,
+                                     get_device=lambda: device, is_contiguous=lambda: True, data_ptr=lambda: 4096)
+
+    ops = _planner()
+    ops._device_index, ops._tickets, ops._quantized_sizes = 0, tensor(torch.int32, 4), {(4, 2, 64, 16)}
+    kv = types.SimpleNamespace(shape=(3, 2, 2, 16, 64), codes=tensor(torch.uint8, 3, 2, 2, 16, 64), scales=tensor(torch.uint8, 3, 2, 2, 16))
+    there = lambda what, n: tensor(torch.float32, n, device=int(what == which))
+    prep = QKPreparation(rotation=Rotation(there("inv_freq", 32)), norm_eps=1e-5, norm_weight_q=there("q norm weight", 64),
+                         norm_weight_k=there("k norm weight", 64))
+    rows, places = tensor(torch.bfloat16, 5, 8 * 64), tensor(torch.int32, 5)
+    with pytest.raises(KernelError, match=which + " must be on the GPU that"):
+        ops._qk_prepare_quantized(rows, 4, 2, 64, places, prep, kv, places)
