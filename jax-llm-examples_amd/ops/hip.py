@@ -2622,12 +2622,14 @@ class HipOps:
             if not 0 < rd <= dh or rd % (16 if pairing else 2):
                 raise KernelError(f"rotary/norm kernel: {rd} rotated elements of a head of {dh} (half-split pairs: a multiple "
                                   "of 16)")
-            self._here(self._chk(inv_freq, torch.float32, (rd // 2,), "inv_freq"), "inv_freq", 4)
+            if self._chk(inv_freq, torch.float32, (rd // 2,), "inv_freq").get_device() != self._device_index:
+                self._here(inv_freq, "inv_freq", 4)
         for w, what in ((prep.norm_weight_q, "q norm weight"), (prep.norm_weight_k, "k norm weight")):
             if w is not None:
                 if prep.norm_eps is None:
                     raise KernelError("rotary/norm kernel: norm weights without a norm")
-                self._here(self._chk(w, torch.float32, (dh,), what), what, 4)
+                if self._chk(w, torch.float32, (dh,), what).get_device() != self._device_index:
+                    self._here(w, what, 4)
         q = torch.empty(n, hq, dh, dtype=qkv.dtype, device=qkv.device)
         fs, sc = (prep.query_scale if prep.query_scale is not None else (0.0, 0.0))
         self._call("jle_quantized_prepare", _p(qkv), _p(q), _p(kv.codes) if writes else None,
@@ -2656,11 +2658,14 @@ class HipOps:
             raise KernelError("no pages to read")
         n = page_ids.numel() if where is None else where.numel()
         first, end = heads or (0, hk)
-        size = n * 2 * (end - first) * ps * dh
-        # (for attention a power of two: a prompt's portions, each with more pages than the last, ask for few different sizes, and
-        # the allocator has what the last one gave back)
-        out = torch.empty(size if where is None else 1 << (size - 1).bit_length(), dtype=torch.bfloat16, device=kv.device)
-        out = out[:size].view(n, 2, end - first, ps, dh)
+        if where is None:
+            out = torch.empty(n, 2, hk, ps, dh, dtype=torch.bfloat16, device=kv.device)
+        else:
+            # a power of two: a prompt's portions, each with more pages than the last, ask for few different sizes, and the
+            # allocator has what the last one gave back
+            size = n * 2 * (end - first) * ps * dh
+            out = torch.empty(1 << (size - 1).bit_length(), dtype=torch.bfloat16, device=kv.device)
+            out = out[:size].view(n, 2, end - first, ps, dh)
         self._call("jle_quantized_read", kv.codes.data_ptr(), kv.scales.data_ptr(), page_ids.data_ptr(), _p(where), out.data_ptr(),
                    n, p, int(where is not None), hk, first, end - first, dh, ps)
         return out

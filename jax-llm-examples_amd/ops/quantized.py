@@ -4,7 +4,8 @@ A token's key (or value) of one kv head is held as e4m3 codes times a power of t
 which the row's largest magnitude stays within 448: ``e = ceil(log2(max |x| / 448))``, at least -126; the scale byte is
 ``e + 127``.  e4m3 rounds relative to a number's own size (half a step is 2^-4 of it; magnitudes below 2^-6 of a code's unit
 are held to 2^-10 of the unit), so a power of two loses nothing against a finer scale, and scaling and its undoing are exact
-(in bfloat16: from 2^-126 on, and below 2^128, which a row's largest numbers may be rounded to from 248 * 2^120 on).  A row that holds something that is no finite number is held as NaN throughout.
+(in bfloat16: from 2^-126 on, and below 2^128, which a row's largest numbers may be rounded to from 248 * 2^120 on).  A row
+that holds something that is no finite number is held as NaN throughout.
 
 The codes of sixteen keys lie together in pieces of 64 elements (a last piece of 32 where 64 does not divide the head), each
 piece in the order in which the lanes of a matrix instruction take it (:func:`places`): every load of the attention kernel
