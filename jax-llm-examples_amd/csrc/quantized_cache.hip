@@ -143,8 +143,8 @@ __device__ __forceinline__ void prepare_head(F (&x)[8], const PrepareArgs& a, co
 // keys, values) a wavefront at a time: a *unit*.  A block takes TB consecutive tokens and forms their sines and cosines once.
 // With one token a block (few tokens) the units are shared out among gridDim.y blocks of four wavefronts and the codes go
 // straight into their pages (one token of 56 heads 4.3 us, 64 of 32 5.2); with several TW wavefronts share a token, the codes
-// are gathered in shared memory and written in larger pieces (8,191 tokens of 48 heads of 128: 48 us, 3.9 TB/s, 98 when every
-// value was stored by itself; vector instructions bound it, 1,850 a token and wavefront): keys eight codes each, the tokens'
+// are gathered in shared memory and written in larger pieces (8,191 tokens of 48 heads of 128: 49 us, 3.8 TB/s, 98 when every
+// value was stored by itself; vector instructions bound it, 1,900 a token and wavefront): keys eight codes each, the tokens'
 // side by side, values the four keys of four elements in 16 bytes where the block's tokens fill an aligned four of a page (other
 // values byte by byte).
 template <int LPH, int TB, int TW>
